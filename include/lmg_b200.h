@@ -271,6 +271,91 @@ int lmg_gather_host(void* dst, size_t dst_bytes, int n, const unsigned long long
 int lmg_sum_types(const float* type_index, const float* type_vector, int n, int ntypes, float* sum,
                   int zerofirst, int* status, void* stream);
 
+/* ---- learned type vectors ---------------------------------------------------------------------
+ * What makes the type vectors that lmg_forward grids out of type indices, for networks that learn them:
+ * rows of a table, their layer norm, dropout, and the gradients back to the table.  The reference has
+ * none of this; a type vector is an input there (include/libmolgrid/coordinateset.h:30-39).
+ *
+ * Vectors are float32, bfloat16 or float16; every product and sum is float32 and a result is rounded
+ * once.  A row has unit stride inside, rows lie `ld` elements apart (ld >= width); elements between
+ * rows are neither read nor written.  Outputs may not overlap inputs, except where a comment allows it. */
+enum { LMG_FLOAT32 = 0, LMG_BFLOAT16 = 1, LMG_FLOAT16 = 2 }; /* of vectors */
+enum { LMG_INDEX_FLOAT32 = 0, LMG_INDEX_INT32 = 1, LMG_INDEX_INT64 = 2 }; /* of type indices */
+
+typedef struct lmg_vectors {
+  void* data;   /* first row */
+  int type;     /* LMG_FLOAT32, LMG_BFLOAT16 or LMG_FLOAT16 */
+  long long ld; /* elements from one row to the next */
+} lmg_vectors;
+
+/* The slots of a batch, batch * max_atoms rows (fewer than 2^31).  A slot is empty behind its example's
+ * atom count, and where its type is negative, is no number, or reaches ntypes; the last sets *status. */
+typedef struct lmg_slots {
+  int batch;
+  int max_atoms;
+  const int* n_atoms;     /* [batch] or NULL: all max_atoms */
+  const void* type_index; /* [batch][max_atoms]; floats are rounded, as lmg_backward rounds them */
+  int index_type;         /* LMG_INDEX_* */
+  int* status;            /* device int or NULL: becomes 1 at a type >= ntypes, is left alone otherwise */
+} lmg_slots;
+
+/* Dropout with probability p in [0, 1]: a value stays, times 1 / (1 - p), where its 32 random bits
+ * reach p * 2^32 (rounded), and is 0 elsewhere, whatever it was.  The bits are those of
+ * Philox4x32-10 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011)
+ * with key `seed`: column c of row r takes half word c % 8 of the block at counter (c / 8, r, low word
+ * of `offset`, high word) as its upper 16 bits, and as its lower 16 bits that half word of the block
+ * with the counter's topmost bit set.  They depend on seed, offset, row and column alone, so the
+ * backward pass makes them again and no mask is stored.  offset < 2^63. */
+typedef struct lmg_dropout_spec {
+  double p;
+  unsigned long long seed, offset;
+  const unsigned long long* state; /* device {seed, offset} in place of the two above, or NULL */
+} lmg_dropout_spec;
+
+/* out[slot][width] = scale * table[type of the slot][width], then dropout (drop may be NULL); empty slots
+ * are 0.  A float32 table may have 16-bit outputs; otherwise the two types agree. */
+int lmg_embed_types(const lmg_slots* slots, int ntypes, int width, const lmg_vectors* table, float scale,
+                    const lmg_dropout_spec* drop, const lmg_vectors* out, void* stream);
+
+/* Gradient of lmg_embed_types with respect to the table: table_gradients[type][width] = scale * the sum of
+ * the gradients diff[slot][width] of the type's slots, after the same dropout; types without a slot get 0.
+ * 16-bit gradients may go into a float32 table; otherwise the two types agree.  The slots of a type are
+ * summed in an order fixed by the sizes of the call: the same call has the same bits again. */
+int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, const lmg_vectors* diff, float scale,
+                             const lmg_dropout_spec* drop, const lmg_vectors* table_gradients, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* out = (x - mean) / sqrt(variance + eps) * weight + bias over the `width` values of each row (the
+ * variance is that of the row itself, divided by width); eps > 0.  x and out have the same type,
+ * weight[width] and bias[width] (either may be NULL: 1 and 0) that type or float32.  Rows behind their
+ * example's atom count get 0; of `rows` only batch, max_atoms and n_atoms are read.  stats[row][2], the mean
+ * and 1 / sqrt(variance + eps), is what the backward pass reads; it may be NULL.  out may be x. */
+int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const void* weight, const void* bias,
+                   int weight_type, float eps, const lmg_vectors* out, float* stats, void* stream);
+
+/* Gradients of lmg_layer_norm from diff, that of its output: x_gradients, and weight_gradients[width] and
+ * bias_gradients[width] (either may be NULL), summed over the rows in an order fixed by the sizes of the call.
+ * x, diff and x_gradients have the same type; weight and the gradients of weight and bias have weight_type.  Empty rows get 0 and
+ * add nothing.  x_gradients may be diff. */
+int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors* x, const void* weight,
+                            int weight_type, const float* stats, const lmg_vectors* diff,
+                            const lmg_vectors* x_gradients, void* weight_gradients, void* bias_gradients,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = dropout of x, [rows][width], both of one type.  The gradient is the same call on the gradient.
+ * out may be x. */
+int lmg_dropout(int rows, int width, const lmg_vectors* x, const lmg_dropout_spec* drop, const lmg_vectors* out,
+                void* stream);
+
+/* Takes one draw of a generator that lives on the device: taken = {seed, offset} of state, whose offset
+ * becomes the next.  A captured call takes another draw at every replay. */
+int lmg_dropout_next(unsigned long long* state, unsigned long long* taken, void* stream);
+
+enum { LMG_OP_EMBED_BACKWARD = 16, LMG_OP_LAYER_NORM_BACKWARD = 17 };
+/* Scratch bytes of the two backward passes above for `rows` slots (ntypes counts in the first alone); they
+ * fail with LMG_ERR_WORKSPACE on a smaller one. */
+size_t lmg_vectors_workspace_bytes(int op, int rows, int ntypes, int width);
+
 /* Reads back (synchronising `stream`) the status word that kernels of the last call that used
  * `workspace` wrote: 0, or LMG_ERR_OUT_OF_RANGE / LMG_ERR_INVALID_ARGUMENT when an atom's type
  * index was >= ntypes - the data-dependent checks of src/grid_maker.cpp:172 and :458-460,

@@ -9,6 +9,9 @@ from .api import (GridMaker, GridInterpolater, Transform, Quaternion, float3,  #
                   set_random_seed)
 from .torch_bindings import (Coords2Grid, Coords2GridFunction, BatchedCoords2GridFunction,  # noqa: F401
                              Grid2CoordsGradientFunction)
+from .type_vectors import (embed_types, embed_types_backward, layer_norm, layer_norm_backward, dropout,  # noqa: F401
+                           generator_state, next_draw, TypeVectors, LayerNorm, Dropout, EmbedTypesFunction,
+                           LayerNormFunction, DropoutFunction)
 from .grids import *  # noqa: F401,F403  Grid1f..Grid8dCUDA, MGrid1f..MGrid8d, set/get_gpu_enabled, ...
 from .grids import __all__ as _grid_names
 from .coordinates import CoordinateSet, Example, ExampleVec  # noqa: F401
@@ -22,6 +25,9 @@ from . import _cabi  # noqa: F401
 
 __all__ = ["GridMaker", "GridInterpolater", "Transform", "Quaternion", "float3", "set_random_seed",
            "Coords2Grid", "Coords2GridFunction", "BatchedCoords2GridFunction", "Grid2CoordsGradientFunction",
+           "embed_types", "embed_types_backward", "layer_norm", "layer_norm_backward", "dropout",
+           "generator_state", "next_draw", "TypeVectors", "LayerNorm", "Dropout", "EmbedTypesFunction",
+           "LayerNormFunction", "DropoutFunction",
            "CoordinateSet", "Example", "ExampleVec", "GninaIndexTyper", "FileAtomMapper",
            "FileMappedGninaTyper", "NullIndexTyper", "default_receptor_typer", "default_ligand_typer",
            "defaultGninaReceptorTyper", "defaultGninaLigandTyper", "CoordCache",

@@ -53,12 +53,34 @@ class RecordSetStruct(ctypes.Structure):
 
 RECORD_TYPES = 28
 
+FLOAT32, BFLOAT16, FLOAT16 = range(3)                    # elements of vectors
+INDEX_FLOAT32, INDEX_INT32, INDEX_INT64 = range(3)       # type indices
+OP_EMBED_BACKWARD, OP_LAYER_NORM_BACKWARD = 16, 17
+
+
+class VectorsStruct(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_int), ("ld", ctypes.c_longlong)]
+
+
+class SlotsStruct(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int), ("max_atoms", ctypes.c_int), ("n_atoms", ctypes.c_void_p),
+                ("type_index", ctypes.c_void_p), ("index_type", ctypes.c_int), ("status", ctypes.c_void_p)]
+
+
+class DropoutStruct(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_ulonglong), ("offset", ctypes.c_ulonglong),
+                ("state", ctypes.c_void_p)]
+
+
 # every symbol include/lmg_b200.h declares: (name, restype, argtypes)
 _VP = ctypes.c_void_p
 _GM = ctypes.POINTER(GridMakerStruct)
 _AT = ctypes.POINTER(AtomsStruct)
 _TR = ctypes.POINTER(TransformStruct)
 _GI = ctypes.POINTER(InterpolaterStruct)
+_VE = ctypes.POINTER(VectorsStruct)
+_SL = ctypes.POINTER(SlotsStruct)
+_DR = ctypes.POINTER(DropoutStruct)
 SYMBOLS = [
     ("lmg_gridmaker_init", ctypes.c_int, [_GM, ctypes.c_float, ctypes.c_float, ctypes.c_int, ctypes.c_int,
                                           ctypes.c_float, ctypes.c_float]),
@@ -88,6 +110,15 @@ SYMBOLS = [
                                           ctypes.c_int, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
     ("lmg_gather_host", ctypes.c_int, [_VP, ctypes.c_size_t, ctypes.c_int, _VP, _VP]),
     ("lmg_sum_types", ctypes.c_int, [_VP, _VP, ctypes.c_int, ctypes.c_int, _VP, ctypes.c_int, _VP, _VP]),
+    ("lmg_embed_types", ctypes.c_int, [_SL, ctypes.c_int, ctypes.c_int, _VE, ctypes.c_float, _DR, _VE, _VP]),
+    ("lmg_embed_types_backward", ctypes.c_int, [_SL, ctypes.c_int, ctypes.c_int, _VE, ctypes.c_float, _DR, _VE, _VP,
+                                                ctypes.c_size_t, _VP]),
+    ("lmg_layer_norm", ctypes.c_int, [_SL, ctypes.c_int, _VE, _VP, _VP, ctypes.c_int, ctypes.c_float, _VE, _VP, _VP]),
+    ("lmg_layer_norm_backward", ctypes.c_int, [_SL, ctypes.c_int, _VE, _VP, ctypes.c_int, _VP, _VE, _VE, _VP, _VP,
+                                               _VP, ctypes.c_size_t, _VP]),
+    ("lmg_dropout", ctypes.c_int, [ctypes.c_int, ctypes.c_int, _VE, _DR, _VE, _VP]),
+    ("lmg_dropout_next", ctypes.c_int, [_VP, _VP, _VP]),
+    ("lmg_vectors_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     ("lmg_check_status", ctypes.c_int, [_VP, _VP]),
     ("lmg_last_error", ctypes.c_char_p, []),
     ("lmg_version", ctypes.c_int, []),

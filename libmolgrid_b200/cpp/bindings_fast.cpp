@@ -312,6 +312,264 @@ PyObject* fast_gradients(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   }(), ret);
 }
 
+// ---- type vectors ---------------------------------------------------------------------------------------------------
+// A CUDA tensor on the current device, any strides: `type` is its LMG_* element type, -1 where it has none.
+struct View {
+  void* ptr = nullptr;
+  int type = -1, index_type = -1, ndim = 0;
+  long long shape[8], stride[8], numel = 1;
+  bool contiguous = false, i32 = false, i64 = false;
+};
+
+bool view(PyObject* o, int device, View& v) try {
+  if (!THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.is_nested() || t.layout() != at::kStrided || !t.is_cuda() || (int)t.get_device() != device || t.dim() > 8) return false;
+  switch (t.scalar_type()) {
+    case at::kFloat: v.type = LMG_FLOAT32, v.index_type = LMG_INDEX_FLOAT32; break;
+    case at::kBFloat16: v.type = LMG_BFLOAT16; break;
+    case at::kHalf: v.type = LMG_FLOAT16; break;
+    case at::kInt: v.index_type = LMG_INDEX_INT32, v.i32 = true; break;
+    case at::kLong: v.index_type = LMG_INDEX_INT64, v.i64 = true; break;
+    default: return false;
+  }
+  v.ndim = (int)t.dim();
+  for (int i = 0; i < v.ndim; i++) v.shape[i] = t.size(i), v.stride[i] = t.stride(i);
+  v.numel = t.numel();
+  v.contiguous = t.is_contiguous();
+  v.ptr = v.numel ? t.data_ptr() : nullptr;
+  return v.ptr != nullptr;  // what is empty goes the general way
+} catch (const std::exception&) {
+  return false;
+}
+
+// rows of vectors, evenly spaced
+bool rows(PyObject* o, int device, View& v, lmg_vectors& r) {
+  if (!view(o, device, v) || v.type < 0 || v.ndim < 1) return false;
+  const int last = v.ndim - 1;
+  long long ld = -1, step = 0;
+  if (v.shape[last] > 1 && v.stride[last] != 1) return false;
+  for (int i = last - 1; i >= 0; i--) {
+    if (v.shape[i] == 1) continue;
+    if (ld < 0) ld = step = v.stride[i];
+    else if (v.stride[i] != step) return false;
+    step *= v.shape[i];
+  }
+  if (ld < 0) ld = v.shape[last];
+  if (ld < v.shape[last] || v.shape[last] >= 0x7fffffff) return false;
+  r.data = v.ptr;
+  r.type = v.type;
+  r.ld = ld;
+  return true;
+}
+
+bool same_shape(const View& a, const View& b) {
+  if (a.ndim != b.ndim) return false;
+  for (int i = 0; i < a.ndim; i++)
+    if (a.shape[i] != b.shape[i]) return false;
+  return true;
+}
+
+// the slots of an array whose first `lead` dimensions are v's, with counts or without
+bool slots(const View& v, int lead, PyObject* n_atoms, int device, lmg_slots& s) {
+  long long n = 1;
+  for (int i = 0; i < lead; i++) n *= v.shape[i];
+  if (n >= 0x7fffffff) return false;
+  s = {};
+  s.batch = 1;
+  s.max_atoms = (int)n;
+  if (n_atoms == Py_None) return true;
+  View c;
+  if (lead != 2 || !view(n_atoms, device, c) || !c.i32 || !c.contiguous || c.ndim != 1 || c.shape[0] != v.shape[0]) return false;
+  s.batch = (int)v.shape[0];
+  s.max_atoms = (int)v.shape[1];
+  s.n_atoms = static_cast<const int*>(c.ptr);
+  return true;
+}
+
+bool type_slots(PyObject* types, PyObject* n_atoms, PyObject* status, int device, View& t, lmg_slots& s) {
+  if (!view(types, device, t) || t.index_type < 0 || !t.contiguous || !slots(t, t.ndim, n_atoms, device, s)) return false;
+  s.type_index = t.ptr;
+  s.index_type = t.index_type;
+  if (status == Py_None) return true;
+  View c;
+  if (!view(status, device, c) || !c.i32 || c.numel != 1) return false;
+  s.status = static_cast<int*>(c.ptr);
+  return true;
+}
+
+bool real(PyObject* o, double* d) {
+  if (PyFloat_CheckExact(o)) *d = PyFloat_AS_DOUBLE(o);
+  else if (PyLong_CheckExact(o)) *d = PyLong_AsDouble(o);
+  else return false;
+  if (PyErr_Occurred() == nullptr) return true;
+  PyErr_Clear();
+  return false;
+}
+
+bool word(PyObject* o, unsigned long long* w) {
+  if (!PyLong_CheckExact(o)) return false;
+  *w = PyLong_AsUnsignedLongLong(o);
+  if (PyErr_Occurred() == nullptr) return true;
+  PyErr_Clear();
+  return false;
+}
+
+bool drop(PyObject* p, PyObject* rng, int device, lmg_dropout_spec& d) {
+  d = {};
+  if (!real(p, &d.p) || !(d.p >= 0.0 && d.p <= 1.0)) return false;
+  if (d.p == 0.0) return true;
+  View v;
+  if (PyTuple_CheckExact(rng))
+    return PyTuple_GET_SIZE(rng) == 2 && word(PyTuple_GET_ITEM(rng, 0), &d.seed) && word(PyTuple_GET_ITEM(rng, 1), &d.offset) && !(d.offset >> 63);
+  if (!view(rng, device, v) || !v.i64 || !v.contiguous || v.ndim != 1 || v.shape[0] != 2) return false;
+  d.state = static_cast<const unsigned long long*>(v.ptr);
+  return true;
+}
+
+// a parameter of `width` values, float32 or of the vectors' type; `type` is that of all parameters so far
+bool parameter(PyObject* o, int device, long long width, int vectors, int& type, void** ptr) {
+  *ptr = nullptr;
+  if (o == Py_None) return true;
+  View v;
+  if (!view(o, device, v) || (v.type != LMG_FLOAT32 && v.type != vectors) || !v.contiguous || v.ndim != 1 || v.shape[0] != width) return false;
+  if (type >= 0 && type != v.type) return false;
+  type = v.type;
+  *ptr = v.ptr;
+  return true;
+}
+
+bool stats_of(PyObject* o, int device, const View& x, float** ptr) {
+  View v;
+  if (!view(o, device, v) || v.type != LMG_FLOAT32 || !v.contiguous || v.ndim != x.ndim || v.shape[v.ndim - 1] != 2) return false;
+  for (int i = 0; i < x.ndim - 1; i++)
+    if (v.shape[i] != x.shape[i]) return false;
+  *ptr = static_cast<float*>(v.ptr);
+  return true;
+}
+
+// torch's stream of the device, and the stream's workspace where there is one of that size
+bool workspace_of(PyObject* workspaces, int device, size_t bytes, Call& c, void** ws, size_t* ws_bytes, cudaStream_t* st, PyObject** ret) {
+  c.workspaces = workspaces;
+  c.device = device;
+  return workspaces != Py_None && place(c, bytes, bytes, ws, ws_bytes, st, ret);
+}
+
+// (types, table, out, scale, n_atoms, p, rng, status)
+PyObject* fast_embed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int device;
+  View t, tab, o;
+  lmg_slots s;
+  lmg_vectors table, out;
+  lmg_dropout_spec d;
+  float scale;
+  if (n != 8 || cudaGetDevice(&device) != cudaSuccess || !type_slots(a[0], a[4], a[7], device, t, s) || !rows(a[1], device, tab, table) ||
+      tab.ndim != 2 || !rows(a[2], device, o, out) || !number(a[3], &scale) || !drop(a[5], a[6], device, d))
+    Py_RETURN_NONE;
+  if (o.ndim != t.ndim + 1 || o.shape[t.ndim] != tab.shape[1] || tab.shape[0] >= 0x7fffffff) Py_RETURN_NONE;
+  for (int i = 0; i < t.ndim; i++)
+    if (o.shape[i] != t.shape[i]) Py_RETURN_NONE;
+  const cudaStream_t st = torch_stream(device);
+  return finish([&] {
+    Released r;
+    return lmg_embed_types(&s, (int)tab.shape[0], (int)tab.shape[1], &table, scale, d.p > 0 ? &d : nullptr, &out, st);
+  }(), Py_NewRef(Py_True));
+}
+
+// (types, diff, table_gradients, scale, n_atoms, p, rng, status, workspaces)
+PyObject* fast_embed_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int device;
+  View t, dv, gv;
+  lmg_slots s;
+  lmg_vectors diff, grad;
+  lmg_dropout_spec d;
+  float scale;
+  if (n != 9 || cudaGetDevice(&device) != cudaSuccess || !type_slots(a[0], a[4], a[7], device, t, s) || !rows(a[1], device, dv, diff) ||
+      !rows(a[2], device, gv, grad) || gv.ndim != 2 || !number(a[3], &scale) || !drop(a[5], a[6], device, d))
+    Py_RETURN_NONE;
+  if (dv.ndim != t.ndim + 1 || dv.shape[t.ndim] != gv.shape[1] || gv.shape[0] >= 0x7fffffff) Py_RETURN_NONE;
+  for (int i = 0; i < t.ndim; i++)
+    if (dv.shape[i] != t.shape[i]) Py_RETURN_NONE;
+  Call c;
+  void* ws;
+  size_t wb;
+  cudaStream_t st;
+  PyObject* ret;
+  const int V = (int)gv.shape[0], W = (int)gv.shape[1];
+  if (!workspace_of(a[8], device, lmg_vectors_workspace_bytes(LMG_OP_EMBED_BACKWARD, s.batch * s.max_atoms, V, W), c, &ws, &wb, &st, &ret))
+    Py_RETURN_NONE;
+  return finish([&] {
+    Released r;
+    return lmg_embed_types_backward(&s, V, W, &diff, scale, d.p > 0 ? &d : nullptr, &grad, ws, wb, st);
+  }(), ret);
+}
+
+// (x, weight, bias, out, stats, eps, n_atoms)
+PyObject* fast_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int device, type = -1;
+  View xv, ov;
+  lmg_slots s;
+  lmg_vectors x, out;
+  void *w, *b;
+  float *stats = nullptr, eps;
+  if (n != 7 || cudaGetDevice(&device) != cudaSuccess || !rows(a[0], device, xv, x) || !rows(a[3], device, ov, out) || !same_shape(xv, ov))
+    Py_RETURN_NONE;
+  const long long width = xv.shape[xv.ndim - 1];
+  if (!parameter(a[1], device, width, x.type, type, &w) || !parameter(a[2], device, width, x.type, type, &b) ||
+      (a[4] != Py_None && !stats_of(a[4], device, xv, &stats)) || !number(a[5], &eps) || !slots(xv, xv.ndim - 1, a[6], device, s))
+    Py_RETURN_NONE;
+  const cudaStream_t st = torch_stream(device);
+  return finish([&] {
+    Released r;
+    return lmg_layer_norm(&s, (int)width, &x, w, b, type < 0 ? LMG_FLOAT32 : type, eps, &out, stats, st);
+  }(), Py_NewRef(Py_True));
+}
+
+// (x, weight, stats, diff, x_gradients, weight_gradients, bias_gradients, n_atoms, workspaces)
+PyObject* fast_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int device, type = -1;
+  View xv, dv, gv;
+  lmg_slots s;
+  lmg_vectors x, diff, grad;
+  void *w, *dw, *db;
+  float* stats;
+  if (n != 9 || cudaGetDevice(&device) != cudaSuccess || !rows(a[0], device, xv, x) || !rows(a[3], device, dv, diff) || !same_shape(xv, dv) ||
+      !rows(a[4], device, gv, grad) || !same_shape(xv, gv))
+    Py_RETURN_NONE;
+  const long long width = xv.shape[xv.ndim - 1];
+  if (!parameter(a[1], device, width, x.type, type, &w) || !parameter(a[5], device, width, x.type, type, &dw) ||
+      !parameter(a[6], device, width, x.type, type, &db) || !stats_of(a[2], device, xv, &stats) || !slots(xv, xv.ndim - 1, a[7], device, s))
+    Py_RETURN_NONE;
+  Call c;
+  void* ws;
+  size_t wb;
+  cudaStream_t st;
+  PyObject* ret;
+  if (!workspace_of(a[8], device, lmg_vectors_workspace_bytes(LMG_OP_LAYER_NORM_BACKWARD, s.batch * s.max_atoms, 0, (int)width), c, &ws, &wb, &st, &ret))
+    Py_RETURN_NONE;
+  return finish([&] {
+    Released r;
+    return lmg_layer_norm_backward(&s, (int)width, &x, w, type < 0 ? LMG_FLOAT32 : type, stats, &diff, &grad, dw, db, ws, wb, st);
+  }(), ret);
+}
+
+// (x, out, p, rng)
+PyObject* fast_dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int device;
+  View xv, ov;
+  lmg_slots s;
+  lmg_vectors x, out;
+  lmg_dropout_spec d;
+  if (n != 4 || cudaGetDevice(&device) != cudaSuccess || !rows(a[0], device, xv, x) || !rows(a[1], device, ov, out) || !same_shape(xv, ov) ||
+      !drop(a[2], a[3], device, d) || !slots(xv, xv.ndim - 1, Py_None, device, s))
+    Py_RETURN_NONE;
+  const cudaStream_t st = torch_stream(device);
+  return finish([&] {
+    Released r;
+    return lmg_dropout(s.max_atoms, (int)xv.shape[xv.ndim - 1], &x, &d, &out, st);
+  }(), Py_NewRef(Py_True));
+}
+
 // A float attribute (any Python or numpy number) of an object; false with an exception set.
 bool number_of(PyObject* o, PyObject* name, float* f) {
   PyObject* v = PyObject_GetAttr(o, name);
@@ -371,6 +629,11 @@ PyMethodDef methods[] = {
     {"_fast_backward", entry<fast_backward>(), METH_FASTCALL, nullptr},
     {"_fast_relevance", entry<fast_relevance>(), METH_FASTCALL, nullptr},
     {"_fast_gradients", entry<fast_gradients>(), METH_FASTCALL, nullptr},
+    {"_fast_embed", entry<fast_embed>(), METH_FASTCALL, nullptr},
+    {"_fast_embed_backward", entry<fast_embed_backward>(), METH_FASTCALL, nullptr},
+    {"_fast_layer_norm", entry<fast_layer_norm>(), METH_FASTCALL, nullptr},
+    {"_fast_layer_norm_backward", entry<fast_layer_norm_backward>(), METH_FASTCALL, nullptr},
+    {"_fast_dropout", entry<fast_dropout>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

@@ -348,6 +348,8 @@ extern "C" {
 const char* lmg_last_error(void) { return g_err.c_str(); }
 // lets the library's other translation units report through lmg_last_error()
 void lmg_internal_set_error(const char* msg) { g_err = msg ? msg : ""; }
+// and count what they launch
+void lmg_internal_count_launches(long n) { g_launches += n; }
 int lmg_version(void) { return 100; }
 
 void lmg_set_random_seed(unsigned seed) { g_engine.seed(seed); }
