@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblmg_b200.so")
 SOURCES = ["lmg_gridmaker.cu", "lmg_occupancy.cu", "lmg_misc.cu", "lmg_cabi.cu", "lmg_noalloc.cu", "lmg_records.cu",
-           "lmg_embed.cu", "lmg_norm.cu"]
+           "lmg_embed.cu", "lmg_embed_grad.cu", "lmg_norm.cu"]
 HEADERS = ["lmg_device.cuh", "lmg_atoms.cuh", "lmg_launch.h", "lmg_misc.h", "lmg_vectors.h", os.path.join("..", "..", "include", "lmg_b200.h")]
 
 NVCC_FLAGS = [

@@ -1,4 +1,4 @@
-// Type indices to rows of a table, dropout, and the gradient of the table.
+// Type indices to rows of a table, and dropout.
 #include "lmg_vectors.h"
 
 #include <cmath>
@@ -37,6 +37,15 @@ int check_drop(const lmg_dropout_spec* d) {
   if (d == nullptr) return LMG_OK;
   if (!(d->p >= 0.0 && d->p <= 1.0)) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "dropout probability outside [0, 1]");
   if (d->state == nullptr && d->offset >> 63) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "dropout offset of 2^63 and more");
+  return LMG_OK;
+}
+
+int check_index(const lmg_slots* s, int ntypes) {
+  if (ntypes < 0) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "negative size");
+  if (s->index_type < LMG_INDEX_FLOAT32 || s->index_type > LMG_INDEX_INT64)
+    return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "type indices of unknown element type");
+  if (s->type_index == nullptr && s->batch > 0 && s->max_atoms > 0)
+    return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "type indices missing memory");
   return LMG_OK;
 }
 
@@ -86,25 +95,6 @@ __global__ void __launch_bounds__(256) k_rows(Slots S, const T* src, long long s
   }
 }
 
-// a block per type walks all slots in order, its threads the columns
-template <class T, class O>
-__global__ void __launch_bounds__(256) k_type_sums(Slots S, const T* diff, long long diff_ld, O* grad, long long grad_ld, int width,
-                                                   float scale, bool dropping, Drop D) {
-  wait_for_stream();
-  const DropKey K(D);
-  const int type = blockIdx.x;
-  for (int col = threadIdx.x; col < width; col += blockDim.x) {
-    float sum = 0.f;
-    for (unsigned r = 0; r < S.rows; r++) {
-      if (slot_type(S, r) != type) continue;
-      const float v = to_float(diff[(long long)r * diff_ld + col]);
-      if (!dropping) sum += v;
-      else if (kept8(D, K, r, col / 8) >> (col & 7) & 1) sum += v * D.scale;
-    }
-    grad[(long long)type * grad_ld + col] = from_float<O>(sum * scale);
-  }
-}
-
 __global__ void k_next_draw(unsigned long long* state, unsigned long long* taken) {
   wait_for_stream();
   const unsigned long long offset = state[1];
@@ -113,38 +103,15 @@ __global__ void k_next_draw(unsigned long long* state, unsigned long long* taken
   state[1] = (offset + 1) & 0x7fffffffffffffffull;
 }
 
-bool dropping(const Drop& D) { return D.threshold_hi != 0 || D.threshold_lo != 0; }
-
-// F(T, O) for the element types of source and result, which agree or are float32 and 16 bits
-template <class F>
-cudaError_t by_types(int in, int out, F f) {
-  if (in == LMG_FLOAT32 && out == LMG_FLOAT32) return f(float(), float());
-  if (in == LMG_FLOAT32 && out == LMG_BFLOAT16) return f(float(), __nv_bfloat16());
-  if (in == LMG_FLOAT32 && out == LMG_FLOAT16) return f(float(), __half());
-  if (in == LMG_BFLOAT16 && out == LMG_FLOAT32) return f(__nv_bfloat16(), float());
-  if (in == LMG_FLOAT16 && out == LMG_FLOAT32) return f(__half(), float());
-  if (in == LMG_BFLOAT16) return f(__nv_bfloat16(), __nv_bfloat16());
-  return f(__half(), __half());
-}
-
 template <bool LOOKUP>
 cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vectors* out, int width, float scale, const Drop& D,
                         cudaStream_t st) {
   const long long blocks = ((long long)S.rows * width + 255) / 256;
   const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
-  return by_types(src->type, out->type, [&](auto t, auto o) {
+  return by_vector_types(src->type, out->type, [&](auto t, auto o) {
     return launch_early(k_rows<decltype(t), decltype(o), LOOKUP>, grid, 256, 0, st, S, static_cast<const decltype(t)*>(src->data), src->ld,
-                        static_cast<decltype(o)*>(out->data), out->ld, width, scale, dropping(D), D);
+                        static_cast<decltype(o)*>(out->data), out->ld, width, scale, drops(D), D);
   });
-}
-
-int check_index(const lmg_slots* s, int ntypes) {
-  if (ntypes < 0) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "negative size");
-  if (s->index_type < LMG_INDEX_FLOAT32 || s->index_type > LMG_INDEX_INT64)
-    return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "type indices of unknown element type");
-  if (s->type_index == nullptr && s->batch > 0 && s->max_atoms > 0)
-    return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "type indices missing memory");
-  return LMG_OK;
 }
 
 }  // namespace
@@ -192,38 +159,6 @@ int lmg_dropout_next(unsigned long long* state, unsigned long long* taken, void*
   if (state == nullptr || taken == nullptr) return lmg::vectors_fail(LMG_ERR_INVALID_ARGUMENT, "generator state missing memory");
   const cudaError_t e = lmg::launch_early(lmg::k_next_draw, dim3(1), 1, 0, (cudaStream_t)stream, state, taken);
   if (e != cudaSuccess) return lmg::vectors_cuda(e, "taking a draw");
-  lmg_internal_count_launches(1);
-  return LMG_OK;
-}
-
-size_t lmg_embed_backward_bytes(int rows, int ntypes, int width) {
-  (void)rows, (void)ntypes, (void)width;
-  return 256;
-}
-
-int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, const lmg_vectors* diff, float scale,
-                             const lmg_dropout_spec* drop, const lmg_vectors* table_gradients, void* workspace,
-                             size_t workspace_bytes, void* stream) {
-  using namespace lmg;
-  int rc;
-  if ((rc = check_slots(slots, width)) || (rc = check_index(slots, ntypes)) || (rc = check_drop(drop))) return rc;
-  if (ntypes == 0 || width == 0) return LMG_OK;
-  if ((rc = check_vectors(table_gradients, width, "table gradients"))) return rc;
-  lmg_vectors none = *table_gradients;  // gradients of no slots are not read
-  if (slots->batch == 0 || slots->max_atoms == 0) diff = &none;
-  if ((rc = check_vectors(diff, width, "diff"))) return rc;
-  if (diff->type != table_gradients->type && table_gradients->type != LMG_FLOAT32)
-    return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "diff and table gradients differ in type, and the gradients are not float32");
-  const Slots S = to_slots(slots, ntypes);
-  if (workspace == nullptr || workspace_bytes < lmg_embed_backward_bytes((int)S.rows, ntypes, width))
-    return vectors_fail(LMG_ERR_WORKSPACE, "workspace too small for the gradient of a table");
-  const Drop D = to_drop(drop);
-  const cudaError_t e = by_types(diff->type, table_gradients->type, [&](auto t, auto o) {
-    return launch_early(k_type_sums<decltype(t), decltype(o)>, dim3((unsigned)ntypes), 256, 0, (cudaStream_t)stream, S,
-                        static_cast<const decltype(t)*>(diff->data), diff->ld, static_cast<decltype(o)*>(table_gradients->data),
-                        table_gradients->ld, width, scale, dropping(D), D);
-  });
-  if (e != cudaSuccess) return vectors_cuda(e, "gradient of a table");
   lmg_internal_count_launches(1);
   return LMG_OK;
 }

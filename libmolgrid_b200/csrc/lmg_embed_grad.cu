@@ -1,0 +1,517 @@
+// Gradient of a table of type vectors: for each type the sum of its slots' gradients.
+//
+// Few types, many slots each (k_type_tables): a warp keeps a table of its own in shared memory and adds row after row to
+// it, so the gradients are read once, in order; the blocks' tables are summed afterwards.  Otherwise the slots are sorted by
+// type (a stable radix sort, k_sort_count and k_sort_move), and groups of lanes walk equal pieces of the sorted
+// slots (k_type_pieces): a type that lies within a piece is written at once, one that crosses pieces leaves partial
+// sums that k_type_joins adds up.  Equal pieces, not types, because a type can hold one slot or all of them.  No atomics touch
+// a sum: its order is fixed by the sizes alone.
+#include "lmg_vectors.h"
+
+namespace lmg {
+namespace {
+
+// ---- few types --------------------------------------------------------------------------------------------------------
+constexpr int TABLE_WARPS = 8, TABLE_COLS = 32, TABLE_ROWS = 8;  // rows whose loads are in flight together
+
+// a warp takes `per` consecutive slots, a lane one of 32 columns; parts[block][type][width], or `grad` where one block does all
+template <class T, class O, bool DROP>
+__global__ void __launch_bounds__(TABLE_WARPS * 32) k_type_tables(Slots S, unsigned per, const T* diff, long long diff_ld, int width, float* parts,
+                                                                  O* grad, long long grad_ld, float scale, Drop D) {
+  extern __shared__ float tables[];  // [warp][type][32]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, V = S.ntypes;
+  for (int i = threadIdx.x; i < TABLE_WARPS * V * TABLE_COLS; i += blockDim.x) tables[i] = 0.f;
+  __syncthreads();
+  wait_for_stream();
+  const DropKey K(D);
+  float* mine = tables + warp * V * TABLE_COLS + lane;
+  const int col = blockIdx.y * TABLE_COLS + lane;
+  const unsigned begin = min((unsigned long long)(blockIdx.x * TABLE_WARPS + warp) * per, (unsigned long long)S.rows);
+  const unsigned end = min((unsigned long long)begin + per, (unsigned long long)S.rows);
+  for (unsigned r0 = begin; r0 < end; r0 += 32) {
+    const int type = r0 + lane < end ? slot_type(S, r0 + lane) : -1;
+    const T* from = diff + (long long)r0 * diff_ld + col;
+#pragma unroll
+    for (int j0 = 0; j0 < 32; j0 += TABLE_ROWS) {
+      if (r0 + j0 >= end) break;
+      float v[TABLE_ROWS];
+      int t[TABLE_ROWS];
+#pragma unroll
+      for (int j = 0; j < TABLE_ROWS; j++) {
+        t[j] = __shfl_sync(0xffffffffu, type, j0 + j);
+        v[j] = t[j] >= 0 && col < width ? to_float(from[(j0 + j) * diff_ld]) : 0.f;
+      }
+      if (DROP) {
+        // 8 rows of 4 groups of 8 columns: a lane draws for one of them and hands its bits round
+        const unsigned bits = kept8(D, K, r0 + j0 + lane / 4, blockIdx.y * (TABLE_COLS / 8) + lane % 4);
+#pragma unroll
+        for (int j = 0; j < TABLE_ROWS; j++) {
+          const unsigned b = __shfl_sync(0xffffffffu, bits, j * 4 + lane / 8);
+          v[j] = b >> (lane & 7) & 1 ? v[j] * D.scale : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TABLE_ROWS; j++)
+        if (t[j] >= 0) mine[t[j] * TABLE_COLS] += v[j];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < V * TABLE_COLS; i += blockDim.x) {
+    const int c = blockIdx.y * TABLE_COLS + (i & (TABLE_COLS - 1)), t = i / TABLE_COLS;
+    if (c >= width) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < TABLE_WARPS; w++) sum += tables[w * V * TABLE_COLS + i];
+    if (gridDim.x == 1) grad[(long long)t * grad_ld + c] = from_float<O>(sum * scale);
+    else parts[((size_t)blockIdx.x * V + t) * width + c] = sum;
+  }
+}
+
+// the sum of all blocks' tables: 32 values a block, eight threads a value
+template <class O>
+__global__ void __launch_bounds__(256) k_table_sums(const float* parts, int n, int V, int width, O* grad, long long grad_ld, float scale) {
+  __shared__ float s[8][32];
+  wait_for_stream();
+  const size_t M = (size_t)V * width, o = (size_t)blockIdx.x * 32 + threadIdx.x % 32;
+  const int slice = threadIdx.x / 32;
+  float sum = 0.f;
+  if (o < M) {
+#pragma unroll 8
+    for (int p = slice; p < n; p += 8) sum += parts[p * M + o];
+  }
+  s[slice][threadIdx.x % 32] = sum;
+  __syncthreads();
+  if (slice == 0 && o < M) {
+    for (int i = 1; i < 8; i++) sum += s[i][threadIdx.x];
+    grad[(long long)(o / width) * grad_ld + o % width] = from_float<O>(sum * scale);
+  }
+}
+
+// ---- the sort ---------------------------------------------------------------------------------------------------------
+constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_TILE_MOST = 32768, SORT_BITS_MOST = 11;
+
+// what a launch of the sort clears on the way: a share of the table's gradient, with what is idle beside the tiles
+struct Clear {
+  char* p;
+  size_t bytes;  // of the share; 16 bytes each, the first on a boundary
+};
+
+struct SortArgs {
+  Slots S;
+  unsigned tiles, tile;  // tiles of `tile` slots, a multiple of SORT_THREADS
+  int shift, bits;
+  const unsigned *key_in, *row_in;  // null in the first pass, which reads the types themselves
+  unsigned *key_out, *row_out;
+  unsigned* counts;  // [tiles][1 << bits]
+  Clear clear;
+};
+
+__device__ __forceinline__ unsigned sort_key(const SortArgs& A, unsigned i) {
+  if (A.key_in != nullptr) return A.key_in[i];
+  const int t = slot_type(A.S, i);
+  return t < 0 ? (unsigned)A.S.ntypes : (unsigned)t;  // empty slots come last
+}
+
+__device__ void clear_share(const Clear& C, unsigned block, unsigned blocks) {
+  uint4* p = reinterpret_cast<uint4*>(C.p);
+  for (size_t i = (size_t)block * SORT_THREADS + threadIdx.x; i < C.bytes / 16; i += (size_t)blocks * SORT_THREADS) p[i] = make_uint4(0, 0, 0, 0);
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(SortArgs A) {
+  __shared__ unsigned count[1 << SORT_BITS_MOST];
+  wait_for_stream();
+  if (blockIdx.x >= A.tiles) return clear_share(A.clear, blockIdx.x - A.tiles, gridDim.x - A.tiles);
+  const unsigned bins = 1u << A.bits;
+  for (unsigned b = threadIdx.x; b < bins; b += SORT_THREADS) count[b] = 0;
+  __syncthreads();
+  const unsigned begin = blockIdx.x * A.tile, end = min(begin + A.tile, A.S.rows);
+  for (unsigned i = begin + threadIdx.x; i < end; i += SORT_THREADS) atomicAdd(&count[sort_key(A, i) >> A.shift & (bins - 1)], 1u);
+  __syncthreads();
+  for (unsigned b = threadIdx.x; b < bins; b += SORT_THREADS) A.counts[(size_t)blockIdx.x * bins + b] = count[b];
+}
+
+// Places of a tile's slots: behind all slots of smaller digits, and those of the same digit in tiles, warps and lanes before.
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_move(SortArgs A) {
+  extern __shared__ unsigned sort_shared[];
+  wait_for_stream();
+  if (blockIdx.x >= A.tiles) return clear_share(A.clear, blockIdx.x - A.tiles, gridDim.x - A.tiles);
+  const unsigned bins = 1u << A.bits, mask = bins - 1, tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+  unsigned* base = sort_shared;                                                         // [bins] first place of a digit's slots here
+  unsigned* total = base + bins;                                                      // [slices][bins]
+  const unsigned slices = bins < SORT_THREADS ? SORT_THREADS / bins : 1;
+  unsigned* before = total + slices * bins;                                           // [slices][bins]
+  unsigned short* mine = reinterpret_cast<unsigned short*>(before + slices * bins) + warp * bins;  // [warps][bins]
+  for (unsigned b = tid; b < slices * bins; b += SORT_THREADS) {
+    unsigned all = 0, earlier = 0;
+#pragma unroll 8
+    for (unsigned t = b / bins; t < A.tiles; t += slices) {
+      const unsigned n = A.counts[(size_t)t * bins + (b & mask)];
+      all += n;
+      earlier += t < blockIdx.x ? n : 0;
+    }
+    total[b] = all;
+    before[b] = earlier;
+  }
+  for (unsigned b = lane; b < bins; b += 32) mine[b] = 0;
+  __syncthreads();
+  // digits' totals to their first places; a thread has two digits at most
+  __shared__ unsigned warp_sum[SORT_WARPS];
+  unsigned sum[2] = {0, 0}, off[2] = {0, 0};
+  const unsigned b0 = bins > SORT_THREADS ? 2 * tid : tid, nb = bins > SORT_THREADS ? 2 : b0 < bins ? 1 : 0;
+  for (unsigned k = 0; k < nb; k++)
+    for (unsigned s = 0; s < slices; s++) {
+      sum[k] += total[s * bins + b0 + k];
+      off[k] += before[s * bins + b0 + k];
+    }
+  unsigned run = sum[0] + sum[1];
+  for (unsigned o = 1; o < 32; o <<= 1) {
+    const unsigned up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 31) warp_sum[warp] = run;
+  __syncthreads();
+  unsigned first = run - sum[0] - sum[1];
+  for (unsigned w = 0; w < warp; w++) first += warp_sum[w];
+  if (nb > 0) base[b0] = first + off[0];
+  if (nb > 1) base[b0 + 1] = first + sum[0] + off[1];
+  // how many of each digit every warp has
+  const unsigned per = A.tile / SORT_WARPS, begin = blockIdx.x * A.tile + warp * per, end = min(begin + per, A.S.rows);
+  for (unsigned i0 = begin; i0 < end; i0 += 32) {
+    const unsigned i = i0 + lane, d = i < end ? sort_key(A, i) >> A.shift & mask : ~0u;
+    const unsigned peers = __match_any_sync(0xffffffffu, d);
+    if (d != ~0u && (peers & ((1u << lane) - 1)) == 0) mine[d] += (unsigned short)__popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  unsigned short* all = reinterpret_cast<unsigned short*>(before + slices * bins);
+  for (unsigned b = tid; b < bins; b += SORT_THREADS) {
+    unsigned at = 0;
+    for (unsigned w = 0; w < SORT_WARPS; w++) {
+      const unsigned n = all[w * bins + b];
+      all[w * bins + b] = (unsigned short)at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  for (unsigned i0 = begin; i0 < end; i0 += 32) {
+    const unsigned i = i0 + lane, key = i < end ? sort_key(A, i) : 0, d = i < end ? key >> A.shift & mask : ~0u;
+    const unsigned peers = __match_any_sync(0xffffffffu, d), lower = peers & ((1u << lane) - 1);
+    const unsigned at = d != ~0u ? base[d] + mine[d] + __popc(lower) : ~0u;
+    __syncwarp();
+    if (d != ~0u && lower == 0) mine[d] += (unsigned short)__popc(peers);
+    __syncwarp();
+    if (at < A.S.rows) {  // always, for types that nobody changes meanwhile
+      A.key_out[at] = key;
+      A.row_out[at] = A.row_in != nullptr ? A.row_in[i] : i;
+    }
+  }
+}
+
+size_t sort_smem(int bits) {
+  const size_t bins = (size_t)1 << bits, slices = bins < SORT_THREADS ? SORT_THREADS / bins : 1;
+  return 4 * bins + 8 * slices * bins + 2 * SORT_WARPS * bins;
+}
+
+// ---- sums of sorted slots ---------------------------------------------------------------------------------------------
+struct PieceArgs {
+  const unsigned *key, *row;
+  unsigned n, ntypes, piece, pieces;
+  int lanes;     // that share a piece, eight columns each; a power of two
+  int width;
+  float* parts;  // [pieces][2][width]: of the type that comes in from the piece before, of the one that goes on in the next
+  float scale;
+};
+
+constexpr int PIECE_THREADS = 256, PIECE_ROWS = 4;
+
+template <class T, class O, bool VEC, bool DROP>
+__global__ void __launch_bounds__(PIECE_THREADS) k_type_pieces(PieceArgs A, const T* diff, long long diff_ld, O* grad, long long grad_ld, Drop D) {
+  wait_for_stream();
+  const unsigned at = blockIdx.x * PIECE_THREADS + threadIdx.x, piece = at / A.lanes;
+  const int col = (blockIdx.y * A.lanes + at % A.lanes) * 8;
+  if (piece >= A.pieces || col >= A.width) return;
+  const DropKey K(D);
+  const unsigned begin = piece * A.piece, end = min(begin + A.piece, A.n);
+  const unsigned came = begin > 0 ? A.key[begin - 1] : ~0u, goes = end < A.n ? A.key[end] : ~0u;
+  float sum[8] = {};
+  unsigned type = A.key[begin];
+  bool first = true;
+  auto put = [&](bool last) {
+    if (type >= A.ntypes) return;
+    if (first && type == came) {
+      store8<float, false>(A.parts + (size_t)piece * 2 * A.width, col, A.width, sum);
+    } else if (last && type == goes) {
+      store8<float, false>(A.parts + ((size_t)piece * 2 + 1) * A.width, col, A.width, sum);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 8; c++) sum[c] *= A.scale;
+      store8<O, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
+    }
+  };
+  for (unsigned i = begin; i < end; i += PIECE_ROWS) {
+    unsigned t[PIECE_ROWS], r[PIECE_ROWS];
+    float v[PIECE_ROWS][8];
+#pragma unroll
+    for (int j = 0; j < PIECE_ROWS; j++) {
+      t[j] = i + j < end ? A.key[i + j] : A.ntypes;
+      r[j] = i + j < end ? A.row[i + j] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < PIECE_ROWS; j++)
+      if (t[j] < A.ntypes) load8<T, VEC>(diff + (long long)r[j] * diff_ld, col, A.width, v[j]);
+#pragma unroll
+    for (int j = 0; j < PIECE_ROWS; j++) {
+      if (i + j >= end) break;
+      if (t[j] != type) {
+        put(false);
+        first = false;
+        type = t[j];
+#pragma unroll
+        for (int c = 0; c < 8; c++) sum[c] = 0.f;
+      }
+      if (type >= A.ntypes) continue;
+      const unsigned keep = DROP ? kept8(D, K, r[j], col / 8) : 0xff;
+#pragma unroll
+      for (int c = 0; c < 8; c++) sum[c] += DROP ? (keep >> c & 1 ? v[j][c] * D.scale : 0.f) : v[j][c];
+    }
+  }
+  put(true);
+}
+
+// a type that begins in a piece and goes on: its parts, piece after piece
+template <class O, bool VEC>
+__global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* grad, long long grad_ld) {
+  wait_for_stream();
+  const unsigned at = blockIdx.x * PIECE_THREADS + threadIdx.x, piece = at / A.lanes;
+  const int col = (blockIdx.y * A.lanes + at % A.lanes) * 8;
+  if (piece + 1 >= A.pieces || col >= A.width) return;
+  const unsigned begin = piece * A.piece, end = begin + A.piece, type = A.key[end - 1];
+  if (type >= A.ntypes || A.key[end] != type || (begin > 0 && A.key[begin - 1] == type)) return;
+  float sum[8];
+  load8<float, false>(A.parts + ((size_t)piece * 2 + 1) * A.width, col, A.width, sum);
+  unsigned p = piece + 1;
+  while (p + 4 <= A.pieces && A.key[(p + 3) * A.piece] == type) {
+    float v[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) load8<float, false>(A.parts + (size_t)(p + j) * 2 * A.width, col, A.width, v[j]);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int c = 0; c < 8; c++) sum[c] += v[j][c];
+    p += 4;
+  }
+  for (; p < A.pieces && A.key[p * A.piece] == type; p++) {
+    float v[8];
+    load8<float, false>(A.parts + (size_t)p * 2 * A.width, col, A.width, v);
+#pragma unroll
+    for (int c = 0; c < 8; c++) sum[c] += v[c];
+  }
+#pragma unroll
+  for (int c = 0; c < 8; c++) sum[c] *= A.scale;
+  store8<O, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
+}
+
+// ---- the plan: a function of the sizes alone, so that the workspace and the call agree ----------------------------------------
+struct Plan {
+  bool tables;
+  // few types
+  unsigned blocks, per;
+  size_t table_smem;
+  // sorted
+  unsigned tiles, tile;
+  int passes, bits;
+  unsigned piece, pieces;
+  int lanes;
+  size_t key[2], row[2], counts, parts, bytes;
+};
+
+constexpr size_t TABLE_SMEM_MOST = 200 << 10;
+
+Plan plan_for(unsigned rows, int V, int width) {
+  Plan p = {};
+  const unsigned col_tiles = (width + TABLE_COLS - 1) / TABLE_COLS;
+  p.table_smem = (size_t)TABLE_WARPS * V * TABLE_COLS * 4;
+  if (V == 0 || width == 0 || rows == 0) {
+    p.tables = true;
+    p.blocks = 1;
+    p.per = 32;
+    p.bytes = 256;
+    return p;
+  }
+  if (p.table_smem <= TABLE_SMEM_MOST) {
+    const unsigned resident = 148 * (unsigned)(p.table_smem * 8 <= 220 << 10 ? 8 : (220 << 10) / (p.table_smem + 1024));
+    unsigned blocks = resident / col_tiles > 0 ? resident / col_tiles : 1;
+    const unsigned most = (rows + TABLE_WARPS * 32 - 1) / (TABLE_WARPS * 32);  // 32 slots a warp
+    if (blocks > most) blocks = most;
+    // the blocks' tables are written and read once more: worth it while they are a fraction of the gradients
+    if ((size_t)blocks * V <= rows || blocks == 1) {
+      p.tables = true;
+      const unsigned warps = blocks * TABLE_WARPS;
+      p.per = ((rows + warps - 1) / warps + 31) / 32 * 32;
+      p.blocks = (rows + p.per * TABLE_WARPS - 1) / (p.per * TABLE_WARPS);
+      p.bytes = 256 + (size_t)p.blocks * V * width * 4;
+      return p;
+    }
+  }
+  p.tile = SORT_THREADS;
+  while ((rows + p.tile - 1) / p.tile > 148 && p.tile < SORT_TILE_MOST) p.tile += SORT_THREADS;
+  p.tiles = (rows + p.tile - 1) / p.tile;
+  int key_bits = 1, most = 1;
+  while (key_bits < 31 && (unsigned)V >> key_bits) key_bits++;
+  // a block reads all tiles' counts: half a megabyte at most
+  while (most < SORT_BITS_MOST && ((size_t)p.tiles << (most + 1)) <= 1 << 17) most++;
+  p.passes = (key_bits + most - 1) / most;
+  p.bits = (key_bits + p.passes - 1) / p.passes;
+  p.lanes = 1;
+  while (p.lanes < 32 && p.lanes * 8 < width) p.lanes *= 2;
+  const unsigned cols = (width + p.lanes * 8 - 1) / (p.lanes * 8);
+  // pieces for 32 warps an SM, of 8 to 256 slots
+  const size_t want = (size_t)rows * cols * p.lanes / (148 * 32 * 32);
+  p.piece = 8;
+  while (p.piece < 256 && p.piece < want) p.piece *= 2;
+  p.pieces = (rows + p.piece - 1) / p.piece;
+  size_t at = 256;
+  for (int k = 0; k < 2; k++) {
+    p.key[k] = at;
+    at += aligned256((size_t)rows * 4);
+    p.row[k] = at;
+    at += aligned256((size_t)rows * 4);
+  }
+  p.counts = at;
+  at += aligned256(((size_t)p.tiles << p.bits) * 4);
+  p.parts = at;
+  at += (size_t)p.pieces * 2 * width * 4;
+  p.bytes = at;
+  return p;
+}
+
+// more shared memory than a launch has without asking, once for each kernel and device
+template <class... P>
+cudaError_t allow_smem(void (*kernel)(P...), size_t bytes) {
+  if (bytes <= 48 << 10) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <class T, class O>
+cudaError_t by_tables(const Slots& S, const Plan& p, const lmg_vectors* diff, const lmg_vectors* grad, int width, float scale, const Drop& D,
+                      char* ws, long* launches, cudaStream_t st) {
+  float* parts = reinterpret_cast<float*>(ws + 256);
+  O* g = static_cast<O*>(grad->data);
+  const auto kernel = drops(D) ? k_type_tables<T, O, true> : k_type_tables<T, O, false>;
+  cudaError_t e = allow_smem(kernel, p.table_smem);
+  if (e == cudaSuccess)
+    e = launch_early(kernel, dim3(p.blocks, (width + TABLE_COLS - 1) / TABLE_COLS), TABLE_WARPS * 32, p.table_smem, st, S, p.per,
+                     static_cast<const T*>(diff->data), diff->ld, width, parts, g, grad->ld, scale, D);
+  if (e != cudaSuccess) return e;
+  ++*launches;
+  if (p.blocks == 1) return e;
+  ++*launches;
+  return launch_early(k_table_sums<O>, dim3((unsigned)(((size_t)S.ntypes * width + 31) / 32)), 256, 0, st, parts, (int)p.blocks, S.ntypes, width, g,
+                      grad->ld, scale);
+}
+
+template <class T, class O>
+cudaError_t by_sort(const Slots& S, const Plan& p, const lmg_vectors* diff, const lmg_vectors* grad, int width, float scale, const Drop& D,
+                    char* ws, long* launches, cudaStream_t st) {
+  // the table's gradient is cleared meanwhile, in shares of the sort's launches; where rows have gaps, or begin off 16 bytes, before
+  const size_t size = sizeof(O), total = (size_t)S.ntypes * width * size;
+  char* g = static_cast<char*>(grad->data);
+  cudaError_t e = cudaSuccess;
+  const bool dense = grad->ld == width && reinterpret_cast<uintptr_t>(g) % 16 == 0;
+  if (!dense) e = cudaMemset2DAsync(g, grad->ld * size, 0, width * size, S.ntypes, st);
+  else if (total % 16) e = cudaMemsetAsync(g + total / 16 * 16, 0, total % 16, st);
+  if (e != cudaSuccess) return e;
+  const int parts = 2 * p.passes;
+  const size_t share = dense ? (total / 16 + parts - 1) / parts * 16 : 0;
+  SortArgs A = {};
+  A.S = S;
+  A.tiles = p.tiles;
+  A.tile = p.tile;
+  A.bits = p.bits;
+  A.counts = reinterpret_cast<unsigned*>(ws + p.counts);
+  const size_t smem = sort_smem(p.bits);
+  if ((e = allow_smem(k_sort_move, smem)) != cudaSuccess) return e;
+  auto clear = [&](int k) {
+    const size_t from = share * k < total / 16 * 16 ? share * k : total / 16 * 16;
+    A.clear.p = g + from;
+    A.clear.bytes = total / 16 * 16 - from < share ? total / 16 * 16 - from : share;
+    const size_t blocks = (A.clear.bytes / 16 + SORT_THREADS * 4 - 1) / (SORT_THREADS * 4);
+    return p.tiles + (unsigned)(blocks < 296 ? blocks : 296);
+  };
+  for (int k = 0; k < p.passes; k++) {
+    A.shift = k * p.bits;
+    A.key_in = k ? reinterpret_cast<unsigned*>(ws + p.key[(k - 1) & 1]) : nullptr;
+    A.row_in = k ? reinterpret_cast<unsigned*>(ws + p.row[(k - 1) & 1]) : nullptr;
+    A.key_out = reinterpret_cast<unsigned*>(ws + p.key[k & 1]);
+    A.row_out = reinterpret_cast<unsigned*>(ws + p.row[k & 1]);
+    unsigned blocks = clear(2 * k);
+    if ((e = launch_early(k_sort_count, dim3(blocks), SORT_THREADS, 0, st, A)) != cudaSuccess) return e;
+    blocks = clear(2 * k + 1);
+    if ((e = launch_early(k_sort_move, dim3(blocks), SORT_THREADS, smem, st, A)) != cudaSuccess) return e;
+    *launches += 2;
+  }
+  PieceArgs P = {};
+  P.key = A.key_out;
+  P.row = A.row_out;
+  P.n = S.rows;
+  P.ntypes = (unsigned)S.ntypes;
+  P.piece = p.piece;
+  P.pieces = p.pieces;
+  P.lanes = p.lanes;
+  P.width = width;
+  P.parts = reinterpret_cast<float*>(ws + p.parts);
+  P.scale = scale;
+  const bool vec = rows_aligned(diff) && rows_aligned(grad);
+  const dim3 grid((unsigned)(((size_t)p.pieces * p.lanes + PIECE_THREADS - 1) / PIECE_THREADS), (width + p.lanes * 8 - 1) / (p.lanes * 8));
+  const auto pieces = vec ? (drops(D) ? k_type_pieces<T, O, true, true> : k_type_pieces<T, O, true, false>)
+                          : (drops(D) ? k_type_pieces<T, O, false, true> : k_type_pieces<T, O, false, false>);
+  e = launch_early(pieces, grid, PIECE_THREADS, 0, st, P, static_cast<const T*>(diff->data), diff->ld, static_cast<O*>(grad->data), grad->ld, D);
+  if (e != cudaSuccess) return e;
+  ++*launches;
+  if (p.pieces == 1) return e;
+  ++*launches;
+  return launch_early(vec ? k_type_joins<O, true> : k_type_joins<O, false>, grid, PIECE_THREADS, 0, st, P, static_cast<O*>(grad->data), grad->ld);
+}
+
+}  // namespace
+}  // namespace lmg
+
+extern "C" {
+
+int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, const lmg_vectors* diff, float scale,
+                             const lmg_dropout_spec* drop, const lmg_vectors* table_gradients, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  using namespace lmg;
+  int rc;
+  if ((rc = check_slots(slots, width)) || (rc = check_index(slots, ntypes)) || (rc = check_drop(drop))) return rc;
+  if (ntypes == 0 || width == 0) return LMG_OK;
+  if ((rc = check_vectors(table_gradients, width, "table gradients"))) return rc;
+  const bool none = slots->batch == 0 || slots->max_atoms == 0;
+  if (!none && (rc = check_vectors(diff, width, "diff"))) return rc;
+  if (!none && diff->type != table_gradients->type && table_gradients->type != LMG_FLOAT32)
+    return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "diff and table gradients differ in type, and the gradients are not float32");
+  const Slots S = to_slots(slots, ntypes);
+  const Plan p = plan_for(S.rows, ntypes, width);
+  if (workspace == nullptr || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return vectors_fail(LMG_ERR_WORKSPACE, "workspace too small for the gradient of a table, or off 16 bytes");
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (none) {
+    const size_t size = element_bytes(table_gradients->type);
+    const cudaError_t e = cudaMemset2DAsync(table_gradients->data, table_gradients->ld * size, 0, width * size, ntypes, st);
+    return e == cudaSuccess ? LMG_OK : vectors_cuda(e, "gradient of a table");
+  }
+  const Drop D = to_drop(drop);
+  long launches = 0;
+  const cudaError_t e = by_vector_types(diff->type, table_gradients->type, [&](auto t, auto o) {
+    const auto by = p.tables ? by_tables<decltype(t), decltype(o)> : by_sort<decltype(t), decltype(o)>;
+    return by(S, p, diff, table_gradients, width, scale, D, static_cast<char*>(workspace), &launches, st);
+  });
+  lmg_internal_count_launches(launches);
+  return e == cudaSuccess ? LMG_OK : vectors_cuda(e, "gradient of a table");
+}
+
+}  // extern "C"
+
+namespace lmg {
+size_t embed_backward_bytes(unsigned rows, int ntypes, int width) { return plan_for(rows, ntypes, width).bytes; }
+}  // namespace lmg

@@ -116,11 +116,9 @@ int check_weights(int type, int weight_type) {
 
 extern "C" {
 
-size_t lmg_embed_backward_bytes(int rows, int ntypes, int width);
-
 size_t lmg_vectors_workspace_bytes(int op, int rows, int ntypes, int width) {
   if (rows < 0 || ntypes < 0 || width < 0) return 0;
-  return op == LMG_OP_EMBED_BACKWARD ? lmg_embed_backward_bytes(rows, ntypes, width) : 256;
+  return op == LMG_OP_EMBED_BACKWARD ? lmg::embed_backward_bytes((unsigned)rows, ntypes, width) : 256;
 }
 
 int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const void* weight, const void* bias, int weight_type,

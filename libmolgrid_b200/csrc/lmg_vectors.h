@@ -86,6 +86,45 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// eight values of a row from column `col` on, zeros behind its end; VEC: both addresses of 16 bytes that they lie in are aligned
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int col, int width, float (&v)[8]) {
+  if (VEC && col + 8 <= width) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(row + col), b = *reinterpret_cast<const float4*>(row + col + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(row + col);
+      const T* h = reinterpret_cast<const T*>(&a);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = to_float(h[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = col + i < width ? to_float(row[col + i]) : 0.f;
+  }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void store8(T* row, int col, int width, const float (&v)[8]) {
+  if (VEC && col + 8 <= width) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(row + col + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint4 a;
+      T* h = reinterpret_cast<T*>(&a);
+#pragma unroll
+      for (int i = 0; i < 8; i++) h[i] = from_float<T>(v[i]);
+      *reinterpret_cast<uint4*>(row + col) = a;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (col + i < width) row[col + i] = from_float<T>(v[i]);
+  }
+}
+
 // Philox4x32-10: ten rounds of two 32 x 32 -> 64 bit products (Salmon, Moraes, Dror and Shaw, 2011, section 4.3)
 __device__ __forceinline__ uint4 philox(uint4 c, unsigned k0, unsigned k1) {
 #pragma unroll
@@ -144,9 +183,27 @@ int vectors_cuda(cudaError_t e, const char* what);
 int check_slots(const lmg_slots* s, int width);
 int check_vectors(const lmg_vectors* v, int width, const char* name);
 int check_drop(const lmg_dropout_spec* d);
+int check_index(const lmg_slots* s, int ntypes);
 Slots to_slots(const lmg_slots* s, int ntypes);
 Drop to_drop(const lmg_dropout_spec* d);  // threshold_hi and _lo 0: nothing is dropped
+inline bool drops(const Drop& D) { return D.threshold_hi != 0 || D.threshold_lo != 0; }
+size_t embed_backward_bytes(unsigned rows, int ntypes, int width);
+// f(T, O) for the element types of source and result, which agree or are float32 and 16 bits
+template <class F>
+cudaError_t by_vector_types(int in, int out, F f) {
+  if (in == LMG_FLOAT32 && out == LMG_FLOAT32) return f(float(), float());
+  if (in == LMG_FLOAT32 && out == LMG_BFLOAT16) return f(float(), __nv_bfloat16());
+  if (in == LMG_FLOAT32 && out == LMG_FLOAT16) return f(float(), __half());
+  if (in == LMG_BFLOAT16 && out == LMG_FLOAT32) return f(__nv_bfloat16(), float());
+  if (in == LMG_FLOAT16 && out == LMG_FLOAT32) return f(__half(), float());
+  if (in == LMG_BFLOAT16) return f(__nv_bfloat16(), __nv_bfloat16());
+  return f(__half(), __half());
+}
 inline size_t element_bytes(int type) { return type == LMG_FLOAT32 ? 4 : 2; }
+// rows of which any eight columns that begin at a multiple of eight lie on 16 bytes
+inline bool rows_aligned(const lmg_vectors* v) {
+  return reinterpret_cast<uintptr_t>(v->data) % 16 == 0 && v->ld * element_bytes(v->type) % 16 == 0;
+}
 inline size_t aligned256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 }  // namespace lmg
