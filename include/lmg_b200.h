@@ -329,7 +329,7 @@ int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, cons
  * variance is that of the row itself, divided by width); eps > 0.  x and out have the same type,
  * weight[width] and bias[width] (either may be NULL: 1 and 0) that type or float32.  Rows behind their
  * example's atom count get 0; of `rows` only batch, max_atoms and n_atoms are read.  stats[row][2], the mean
- * and 1 / sqrt(variance + eps), is what the backward pass reads; it may be NULL.  out may be x. */
+ * and 1 / sqrt(variance + eps), is what the backward pass reads, on 8 bytes; it may be NULL.  out may be x. */
 int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const void* weight, const void* bias,
                    int weight_type, float eps, const lmg_vectors* out, float* stats, void* stream);
 
@@ -353,7 +353,7 @@ int lmg_dropout_next(unsigned long long* state, unsigned long long* taken, void*
 
 enum { LMG_OP_EMBED_BACKWARD = 16, LMG_OP_LAYER_NORM_BACKWARD = 17 };
 /* Scratch bytes of the two backward passes above for `rows` slots (ntypes counts in the first alone); they
- * fail with LMG_ERR_WORKSPACE on a smaller one. */
+ * fail with LMG_ERR_WORKSPACE on a smaller one, and on one that does not start on 16 bytes. */
 size_t lmg_vectors_workspace_bytes(int op, int rows, int ntypes, int width);
 
 /* Reads back (synchronising `stream`) the status word that kernels of the last call that used
