@@ -77,21 +77,138 @@ Drop to_drop(const lmg_dropout_spec* d) {
 
 namespace {
 
-// out[row][col] = scale * source row's value, dropped.  LOOKUP: the source row is the slot's type's, else the row itself.
-template <class T, class O, bool LOOKUP>
-__global__ void __launch_bounds__(256) k_rows(Slots S, const T* src, long long src_ld, O* out, long long out_ld, int width,
-                                              float scale, bool dropping, Drop D) {
+// A pass over rows first .. first + S.rows of a call, out[row][col] = scale * source row's value, dropped.  The source row is the
+// slot's type's (LOOKUP) or the row itself.
+struct RowArgs {
+  Slots S;
+  unsigned first, rows;
+  int width;
+  FastDiv by_groups, by_width;  // eight columns a group
+  long long src_ld, out_ld;
+  float scale;
+  Drop D;
+};
+
+// Rows on 16 bytes: a thread takes groups of eight columns, which are one block of the generator, `UNITS` of them so that as many
+// chains type -> row -> value are under way.
+template <class T, class O, bool LOOKUP, bool DROP, int UNITS>
+__global__ void __launch_bounds__(256) k_rows_aligned(RowArgs A, const T* src, O* out) {
   wait_for_stream();
-  const DropKey K(D);
-  const long long n = (long long)S.rows * width;
+  const DropKey K(A.D);
+  const unsigned groups = A.by_groups.d, n = A.rows * groups, u0 = blockIdx.x * (256 * UNITS) + threadIdx.x;
+  long long from[UNITS];
+  unsigned row[UNITS];
+  int col[UNITS];
+#pragma unroll
+  for (int k = 0; k < UNITS; k++) {
+    const unsigned u = u0 + 256 * k;
+    const unsigned r = A.by_groups(u < n ? u : 0);
+    row[k] = A.first + r;
+    col[k] = u < n ? (int)(u - r * groups) * 8 : A.width;  // behind the row's end: nothing is loaded or stored
+    from[k] = row[k];
+    if (LOOKUP) from[k] = slot_type(A.S, row[k]);
+  }
+  float v[UNITS][8];
+#pragma unroll
+  for (int k = 0; k < UNITS; k++) {
+    if (!LOOKUP || from[k] >= 0) {
+      load8<T, true>(src + from[k] * A.src_ld, col[k], A.width, v[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[k][i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < UNITS; k++) {
+    if (col[k] >= A.width) continue;
+    const unsigned keep = DROP ? kept8(A.D, K, row[k], col[k] / 8) : 0xff;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (LOOKUP) v[k][i] *= A.scale;
+      if (DROP) v[k][i] = keep >> i & 1 ? v[k][i] * A.D.scale : 0.f;
+    }
+    store8<O, true>(out + (long long)row[k] * A.out_ld, col[k], A.width, v[k]);
+  }
+}
+
+// Rows of any width that follow one another without gaps, from 16 bytes on: a block writes 2048 values, 16 bytes a thread and
+// turn, wherever rows begin and end in them; the types of its rows and the bits of its groups are made once, in shared memory.
+constexpr int FLAT = 2048;
+
+template <class T, class O, bool LOOKUP, bool DROP>
+__global__ void __launch_bounds__(256) k_rows_flat(RowArgs A, const T* src, O* out) {
+  __shared__ unsigned char kept[DROP ? FLAT + 8 : 1];
+  __shared__ int types[LOOKUP ? FLAT + 8 : 1];
+  wait_for_stream();
+  const unsigned n = A.rows * (unsigned)A.width, e0 = blockIdx.x * FLAT, last = min(e0 + FLAT, n) - 1;
+  const unsigned row0 = A.by_width(e0), row1 = A.by_width(last), groups = A.by_groups.d;
+  if (LOOKUP)
+    for (unsigned r = row0 + threadIdx.x; r <= row1; r += 256) types[r - row0] = slot_type(A.S, A.first + r);
+  const unsigned g0 = row0 * groups + (e0 - row0 * A.width) / 8, g1 = row1 * groups + (last - row1 * A.width) / 8;
+  if (DROP) {
+    const DropKey K(A.D);
+    for (unsigned g = g0 + threadIdx.x; g <= g1; g += 256) {
+      const unsigned r = A.by_groups(g);
+      kept[g - g0] = (unsigned char)kept8(A.D, K, A.first + r, g - r * groups);
+    }
+  }
+  if (LOOKUP || DROP) __syncthreads();
+  constexpr int N = 16 / sizeof(O);
+#pragma unroll
+  for (int j = 0; j < FLAT / 256 / N; j++) {
+    const unsigned e = e0 + (j * 256 + threadIdx.x) * N;
+    if (e > last) break;
+    unsigned row = A.by_width(e), col = e - row * A.width;
+    const bool whole = e + N <= n;
+    float v[N];
+    if (!LOOKUP && sizeof(T) == sizeof(O) && whole) {
+      const uint4 a = *reinterpret_cast<const uint4*>(src + (long long)A.first * A.width + e);
+      const T* h = reinterpret_cast<const T*>(&a);
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = to_float(h[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (e + i < n) {
+        if (LOOKUP) {
+          const int t = types[row - row0];
+          v[i] = t >= 0 ? to_float(src[t * A.src_ld + col]) * A.scale : 0.f;
+        } else if (!whole) {
+          v[i] = to_float(src[(long long)A.first * A.width + e + i]);
+        }
+        if (DROP) v[i] = kept[row * groups + col / 8 - g0] >> (col & 7) & 1 ? v[i] * A.D.scale : 0.f;
+        if (++col == (unsigned)A.width) col = 0, row++;
+      }
+    }
+    O* to = out + (long long)A.first * A.width + e;
+    if (whole) {
+      uint4 a;
+      O* h = reinterpret_cast<O*>(&a);
+#pragma unroll
+      for (int i = 0; i < N; i++) h[i] = from_float<O>(v[i]);
+      *reinterpret_cast<uint4*>(to) = a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (e + i < n) to[i] = from_float<O>(v[i]);
+    }
+  }
+}
+
+// everything else: a thread a value
+template <class T, class O, bool LOOKUP>
+__global__ void __launch_bounds__(256) k_rows(RowArgs A, const T* src, O* out, bool dropping) {
+  wait_for_stream();
+  const DropKey K(A.D);
+  const long long n = (long long)A.rows * A.width;
   for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (long long)gridDim.x * blockDim.x) {
-    const unsigned row = (unsigned)(e / width), col = (unsigned)(e - (long long)row * width);
+    const unsigned r = (unsigned)(e / A.width), col = (unsigned)(e - (long long)r * A.width), row = A.first + r;
     long long from = row;
-    if (LOOKUP) from = slot_type(S, row);  // an int: -1 stays negative
+    if (LOOKUP) from = slot_type(A.S, row);  // an int: -1 stays negative
     float v = 0.f;
-    if (from >= 0) v = to_float(src[from * src_ld + col]) * scale;
-    if (dropping) v = kept8(D, K, row, col / 8) >> (col & 7) & 1 ? v * D.scale : 0.f;
-    out[(long long)row * out_ld + col] = from_float<O>(v);
+    if (from >= 0) v = to_float(src[from * A.src_ld + col]) * A.scale;
+    if (dropping) v = kept8(A.D, K, row, col / 8) >> (col & 7) & 1 ? v * A.D.scale : 0.f;
+    out[(long long)row * A.out_ld + col] = from_float<O>(v);
   }
 }
 
@@ -104,13 +221,41 @@ __global__ void k_next_draw(unsigned long long* state, unsigned long long* taken
 }
 
 template <bool LOOKUP>
-cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vectors* out, int width, float scale, const Drop& D,
+cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vectors* out, int width, float scale, const Drop& D, long* launches,
                         cudaStream_t st) {
-  const long long blocks = ((long long)S.rows * width + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+  RowArgs A = {S, 0, S.rows, width, FastDiv((unsigned)((long long)width + 7 >> 3)), FastDiv((unsigned)width), src->ld, out->ld, scale, D};
+  const bool aligned = rows_aligned(src) && rows_aligned(out);
+  const bool flat = out->ld == width && reinterpret_cast<uintptr_t>(out->data) % 16 == 0 &&
+                    (LOOKUP || (src->ld == width && reinterpret_cast<uintptr_t>(src->data) % 16 == 0));
+  // passes of less than 2^30 values, a multiple of eight rows so that each begins on 16 bytes again
+  const unsigned most = width > 1 << 26 ? 0 : (1u << 30) / (unsigned)width & ~7u;
   return by_vector_types(src->type, out->type, [&](auto t, auto o) {
-    return launch_early(k_rows<decltype(t), decltype(o), LOOKUP>, grid, 256, 0, st, S, static_cast<const decltype(t)*>(src->data), src->ld,
-                        static_cast<decltype(o)*>(out->data), out->ld, width, scale, drops(D), D);
+    typedef decltype(t) T;
+    typedef decltype(o) O;
+    const T* from = static_cast<const T*>(src->data);
+    O* to = static_cast<O*>(out->data);
+    cudaError_t e = cudaSuccess;
+    if ((!aligned && !flat) || most == 0) {
+      const long long blocks = ((long long)S.rows * width + 255) / 256;
+      ++*launches;
+      return launch_early(k_rows<T, O, LOOKUP>, dim3((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64)), 256, 0, st, A, from, to, drops(D));
+    }
+    for (A.first = 0; A.first < S.rows && e == cudaSuccess; A.first += A.rows) {
+      A.rows = S.rows - A.first < most ? S.rows - A.first : most;
+      const unsigned units = A.rows * A.by_groups.d;
+      ++*launches;
+      if (!aligned) {
+        e = launch_early(drops(D) ? k_rows_flat<T, O, LOOKUP, true> : k_rows_flat<T, O, LOOKUP, false>,
+                         dim3((unsigned)(((long long)A.rows * width + FLAT - 1) / FLAT)), 256, 0, st, A, from, to);
+      } else if (units <= 148 * 256 * 4) {  // one wave: more threads instead of more units a thread
+        e = launch_early(drops(D) ? k_rows_aligned<T, O, LOOKUP, true, 1> : k_rows_aligned<T, O, LOOKUP, false, 1>, dim3((units + 255) / 256), 256, 0, st,
+                         A, from, to);
+      } else {
+        e = launch_early(drops(D) ? k_rows_aligned<T, O, LOOKUP, true, 4> : k_rows_aligned<T, O, LOOKUP, false, 4>, dim3((units + 1023) / 1024), 256, 0, st,
+                         A, from, to);
+      }
+    }
+    return e;
   });
 }
 
@@ -132,9 +277,10 @@ int lmg_embed_types(const lmg_slots* slots, int ntypes, int width, const lmg_vec
   if ((rc = check_vectors(table, width, "table"))) return rc;
   if (table->type != out->type && table->type != LMG_FLOAT32)
     return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "table and output differ in type, and the table is not float32");
-  const cudaError_t e = launch_rows<true>(to_slots(slots, ntypes), table, out, width, scale, to_drop(drop), (cudaStream_t)stream);
+  long launches = 0;
+  const cudaError_t e = launch_rows<true>(to_slots(slots, ntypes), table, out, width, scale, to_drop(drop), &launches, (cudaStream_t)stream);
+  lmg_internal_count_launches(launches);
   if (e != cudaSuccess) return vectors_cuda(e, "looking up types");
-  lmg_internal_count_launches(1);
   return LMG_OK;
 }
 
@@ -149,9 +295,10 @@ int lmg_dropout(int rows, int width, const lmg_vectors* x, const lmg_dropout_spe
   if (rows == 0 || width == 0) return LMG_OK;
   if ((rc = check_vectors(x, width, "input")) || (rc = check_vectors(out, width, "output"))) return rc;
   if (x->type != out->type) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "input and output differ in type");
-  const cudaError_t e = launch_rows<false>(to_slots(&s, 0), x, out, width, 1.f, to_drop(drop), (cudaStream_t)stream);
+  long launches = 0;
+  const cudaError_t e = launch_rows<false>(to_slots(&s, 0), x, out, width, 1.f, to_drop(drop), &launches, (cudaStream_t)stream);
+  lmg_internal_count_launches(launches);
   if (e != cudaSuccess) return vectors_cuda(e, "dropping values");
-  lmg_internal_count_launches(1);
   return LMG_OK;
 }
 

@@ -86,42 +86,40 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// eight values of a row from column `col` on, zeros behind its end; VEC: both addresses of 16 bytes that they lie in are aligned
+// eight values of a row from column `col` on, zeros behind its end; VEC: column 0 lies on 16 bytes and `col` is a multiple of 8
 template <class T, bool VEC>
 __device__ __forceinline__ void load8(const T* row, int col, int width, float (&v)[8]) {
-  if (VEC && col + 8 <= width) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(row + col), b = *reinterpret_cast<const float4*>(row + col + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  constexpr int N = VEC ? 16 / sizeof(T) : 8;
+#pragma unroll
+  for (int k = 0; k < 8; k += N) {
+    if (VEC && col + k + N <= width) {
+      const uint4 a = *reinterpret_cast<const uint4*>(row + col + k);
+      const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+      for (int i = 0; i < N; i++) v[k + i] = to_float(e[i]);
     } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(row + col);
-      const T* h = reinterpret_cast<const T*>(&a);
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = to_float(h[i]);
+      for (int i = 0; i < N; i++) v[k + i] = col + k + i < width ? to_float(row[col + k + i]) : 0.f;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = col + i < width ? to_float(row[col + i]) : 0.f;
   }
 }
 
 template <class T, bool VEC>
 __device__ __forceinline__ void store8(T* row, int col, int width, const float (&v)[8]) {
-  if (VEC && col + 8 <= width) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(row + col + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
+  constexpr int N = VEC ? 16 / sizeof(T) : 8;
+#pragma unroll
+  for (int k = 0; k < 8; k += N) {
+    if (VEC && col + k + N <= width) {
       uint4 a;
-      T* h = reinterpret_cast<T*>(&a);
+      T* e = reinterpret_cast<T*>(&a);
 #pragma unroll
-      for (int i = 0; i < 8; i++) h[i] = from_float<T>(v[i]);
-      *reinterpret_cast<uint4*>(row + col) = a;
+      for (int i = 0; i < N; i++) e[i] = from_float<T>(v[k + i]);
+      *reinterpret_cast<uint4*>(row + col + k) = a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (col + k + i < width) row[col + k + i] = from_float<T>(v[k + i]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (col + i < width) row[col + i] = from_float<T>(v[i]);
   }
 }
 
@@ -129,9 +127,8 @@ __device__ __forceinline__ void store8(T* row, int col, int width, const float (
 __device__ __forceinline__ uint4 philox(uint4 c, unsigned k0, unsigned k1) {
 #pragma unroll
   for (int i = 0; i < 10; i++) {
-    const unsigned h0 = __umulhi(c.x, 0xD2511F53u), l0 = c.x * 0xD2511F53u;
-    const unsigned h1 = __umulhi(c.z, 0xCD9E8D57u), l1 = c.z * 0xCD9E8D57u;
-    c = make_uint4(h1 ^ c.y ^ k0, l1, h0 ^ c.w ^ k1, l0);
+    const unsigned long long a = (unsigned long long)c.x * 0xD2511F53u, b = (unsigned long long)c.z * 0xCD9E8D57u;
+    c = make_uint4((unsigned)(b >> 32) ^ c.y ^ k0, (unsigned)b, (unsigned)(a >> 32) ^ c.w ^ k1, (unsigned)a);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
