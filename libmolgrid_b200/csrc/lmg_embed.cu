@@ -66,8 +66,8 @@ Drop to_drop(const lmg_dropout_spec* d) {
   Drop D = {};
   if (d == nullptr) return D;
   const unsigned long long t = (unsigned long long)std::llround(d->p * 4294967296.0);
-  D.threshold_hi = (unsigned)(t >> 16);
-  D.threshold_lo = (unsigned)(t & 0xffffu);
+  D.upper = t >> 32 ? 65535u : (unsigned)(t >> 16);
+  D.lower = t >> 32 ? 65536u : (unsigned)(t & 0xffffu);
   D.scale = d->p < 1.0 ? (float)(1.0 / (1.0 - d->p)) : 0.f;
   D.seed = d->seed;
   D.offset = d->offset;
@@ -77,120 +77,142 @@ Drop to_drop(const lmg_dropout_spec* d) {
 
 namespace {
 
-// A pass over rows first .. first + S.rows of a call, out[row][col] = scale * source row's value, dropped.  The source row is the
+// A pass over rows first .. first + rows of a call, out[row][col] = scale * source row's value, dropped.  The source row is the
 // slot's type's (LOOKUP) or the row itself.
 struct RowArgs {
   Slots S;
   unsigned first, rows;
   int width;
-  FastDiv by_groups, by_width;  // eight columns a group
+  unsigned groups, across, down;             // of eight columns a row; a block has `across` x `down` threads at work
+  FastDiv by_groups, by_width, by_across;
   long long src_ld, out_ld;
   float scale;
   Drop D;
 };
 
-// Rows on 16 bytes: a thread takes groups of eight columns, which are one block of the generator, `UNITS` of them so that as many
-// chains type -> row -> value are under way.
-template <class T, class O, bool LOOKUP, bool DROP, int UNITS>
-__global__ void __launch_bounds__(256) k_rows_aligned(RowArgs A, const T* src, O* out) {
+// Rows on 16 bytes: a thread takes COLS columns of UNITS rows, so that as many loads are under way; with dropout eight columns, which are one
+// block of the generator.  The types of a block's rows are looked up once, in shared memory.
+constexpr int UNITS_MOST = 4;
+
+template <class T, class O, bool LOOKUP, bool DROP, int COLS, int UNITS>
+__global__ void __launch_bounds__(256, 6) k_rows_aligned(RowArgs A, const T* src, O* out) {
+  __shared__ int types[LOOKUP ? 256 * UNITS : 1];
   wait_for_stream();
+  const unsigned first = blockIdx.x * (A.down * UNITS);
+  if (LOOKUP) {
+    for (unsigned i = threadIdx.x; i < A.down * UNITS; i += blockDim.x) types[i] = first + i < A.rows ? slot_type(A.S, A.first + first + i) : -1;
+    __syncthreads();
+  }
+  const unsigned sub = A.by_across(threadIdx.x), g = blockIdx.y * A.across + threadIdx.x - sub * A.across;
+  if (sub >= A.down || g >= A.groups) return;
+  const int col = (int)g * COLS;
+  Raw<T, COLS> raw[UNITS];
+#pragma unroll
+  for (int k = 0; k < UNITS; k++) {
+    const unsigned i = sub + k * A.down;
+    const int type = LOOKUP ? types[i] : 0;
+    if (LOOKUP ? type >= 0 : first + i < A.rows) raw[k].load(src + (LOOKUP ? (long long)type : (long long)(A.first + first + i)) * A.src_ld, col, A.width);
+    else raw[k].clear();
+  }
+  const unsigned row = A.first + first + sub;
+  uint4 c[UNITS];
   const DropKey K(A.D);
-  const unsigned groups = A.by_groups.d, n = A.rows * groups, u0 = blockIdx.x * (256 * UNITS) + threadIdx.x;
-  long long from[UNITS];
-  unsigned row[UNITS];
-  int col[UNITS];
+  if (DROP) {
 #pragma unroll
-  for (int k = 0; k < UNITS; k++) {
-    const unsigned u = u0 + 256 * k;
-    const unsigned r = A.by_groups(u < n ? u : 0);
-    row[k] = A.first + r;
-    col[k] = u < n ? (int)(u - r * groups) * 8 : A.width;  // behind the row's end: nothing is loaded or stored
-    from[k] = row[k];
-    if (LOOKUP) from[k] = slot_type(A.S, row[k]);
-  }
-  float v[UNITS][8];
-#pragma unroll
-  for (int k = 0; k < UNITS; k++) {
-    if (!LOOKUP || from[k] >= 0) {
-      load8<T, true>(src + from[k] * A.src_ld, col[k], A.width, v[k]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[k][i] = 0.f;
-    }
+    for (int k = 0; k < UNITS; k++) c[k] = make_uint4(g, row + k * A.down, K.o0, K.o1);
+    philox(c, K.k0, K.k1);
   }
 #pragma unroll
   for (int k = 0; k < UNITS; k++) {
-    if (col[k] >= A.width) continue;
-    const unsigned keep = DROP ? kept8(A.D, K, row[k], col[k] / 8) : 0xff;
+    if (first + sub + k * A.down >= A.rows) break;
+    float v[COLS];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      if (LOOKUP) v[k][i] *= A.scale;
-      if (DROP) v[k][i] = keep >> i & 1 ? v[k][i] * A.D.scale : 0.f;
+    for (int i = 0; i < COLS; i++) v[i] = LOOKUP ? raw[k].get(i) * A.scale : raw[k].get(i);
+    if constexpr (DROP) {
+      Bits8 b;
+      b.set(c[k], A.D, K, row + k * A.down, g);
+      b.apply(A.D.scale, v);
     }
-    store8<O, true>(out + (long long)row[k] * A.out_ld, col[k], A.width, v[k]);
+    store_cols<O, COLS>(out + (long long)(row + k * A.down) * A.out_ld, col, A.width, v);
   }
 }
 
 // Rows of any width that follow one another without gaps, from 16 bytes on: a block writes 2048 values, 16 bytes a thread and
-// turn, wherever rows begin and end in them; the types of its rows and the bits of its groups are made once, in shared memory.
+// turn, wherever rows begin and end in them.  The types of its rows, and which of its values stay, a bit each, are made once,
+// in shared memory.
 constexpr int FLAT = 2048;
 
 template <class T, class O, bool LOOKUP, bool DROP>
 __global__ void __launch_bounds__(256) k_rows_flat(RowArgs A, const T* src, O* out) {
-  __shared__ unsigned char kept[DROP ? FLAT + 8 : 1];
-  __shared__ int types[LOOKUP ? FLAT + 8 : 1];
+  __shared__ unsigned kept[DROP ? FLAT / 32 : 1];
+  __shared__ int types[LOOKUP ? FLAT : 1];
+  const unsigned n = A.rows * (unsigned)A.width, e0 = blockIdx.x * FLAT, end = min(e0 + FLAT, n);
+  const unsigned row0 = A.by_width(e0), row1 = A.by_width(end - 1), groups = A.by_groups.d;
+  if (DROP) {
+    for (int i = threadIdx.x; i < FLAT / 32; i += 256) kept[i] = 0;
+    __syncthreads();
+  }
   wait_for_stream();
-  const unsigned n = A.rows * (unsigned)A.width, e0 = blockIdx.x * FLAT, last = min(e0 + FLAT, n) - 1;
-  const unsigned row0 = A.by_width(e0), row1 = A.by_width(last), groups = A.by_groups.d;
   if (LOOKUP)
     for (unsigned r = row0 + threadIdx.x; r <= row1; r += 256) types[r - row0] = slot_type(A.S, A.first + r);
-  const unsigned g0 = row0 * groups + (e0 - row0 * A.width) / 8, g1 = row1 * groups + (last - row1 * A.width) / 8;
   if (DROP) {
     const DropKey K(A.D);
+    const unsigned g0 = row0 * groups + (e0 - row0 * A.width) / 8, g1 = row1 * groups + (end - 1 - row1 * A.width) / 8;
     for (unsigned g = g0 + threadIdx.x; g <= g1; g += 256) {
-      const unsigned r = A.by_groups(g);
-      kept[g - g0] = (unsigned char)kept8(A.D, K, A.first + r, g - r * groups);
+      const unsigned r = A.by_groups(g), in_row = g - r * groups;
+      unsigned bits = kept8(A.D, K, A.first + r, in_row);
+      if ((in_row + 1) * 8 > (unsigned)A.width) bits &= (1u << (A.width & 7)) - 1;
+      // the group's first value may lie before the block's, its last behind it
+      const int at = (int)(r * (unsigned)A.width + in_row * 8 - e0);
+      const unsigned long long wide = (unsigned long long)bits << (at & 31);
+      const int word = at >> 5;  // -1: the bits that reach into word 0 are those of the upper half
+      if (word >= 0 && (unsigned)wide != 0) atomicOr(&kept[word], (unsigned)wide);
+      if (word + 1 < FLAT / 32 && (unsigned)(wide >> 32) != 0) atomicOr(&kept[word + 1], (unsigned)(wide >> 32));
     }
   }
   if (LOOKUP || DROP) __syncthreads();
   constexpr int N = 16 / sizeof(O);
+  const T* from = src + (LOOKUP ? 0 : (long long)A.first * A.width);
+  O* to = out + (long long)A.first * A.width;
 #pragma unroll
   for (int j = 0; j < FLAT / 256 / N; j++) {
     const unsigned e = e0 + (j * 256 + threadIdx.x) * N;
-    if (e > last) break;
-    unsigned row = A.by_width(e), col = e - row * A.width;
-    const bool whole = e + N <= n;
+    if (e >= end) break;
+    const bool whole = e + N <= end;
     float v[N];
-    if (!LOOKUP && sizeof(T) == sizeof(O) && whole) {
-      const uint4 a = *reinterpret_cast<const uint4*>(src + (long long)A.first * A.width + e);
-      const T* h = reinterpret_cast<const T*>(&a);
+    if (LOOKUP) {
+      unsigned row = A.by_width(e), col = e - row * A.width;
+      if (col + N <= (unsigned)A.width) {  // within a row
+        const int t = types[row - row0];
+        const T* p = from + t * A.src_ld + col;
 #pragma unroll
-      for (int i = 0; i < N; i++) v[i] = to_float(h[i]);
-    }
+        for (int i = 0; i < N; i++) v[i] = t >= 0 ? to_float(p[i]) * A.scale : 0.f;
+      } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      if (e + i < n) {
-        if (LOOKUP) {
+        for (int i = 0; i < N; i++) {
+          if (e + i >= end) break;
           const int t = types[row - row0];
-          v[i] = t >= 0 ? to_float(src[t * A.src_ld + col]) * A.scale : 0.f;
-        } else if (!whole) {
-          v[i] = to_float(src[(long long)A.first * A.width + e + i]);
+          v[i] = t >= 0 ? to_float(from[t * A.src_ld + col]) * A.scale : 0.f;
+          if (++col == (unsigned)A.width) col = 0, row++;
         }
-        if (DROP) v[i] = kept[row * groups + col / 8 - g0] >> (col & 7) & 1 ? v[i] * A.D.scale : 0.f;
-        if (++col == (unsigned)A.width) col = 0, row++;
       }
-    }
-    O* to = out + (long long)A.first * A.width + e;
-    if (whole) {
-      uint4 a;
-      O* h = reinterpret_cast<O*>(&a);
+    } else if (whole) {
+      load_cols<T, N>(from + e, 0, N, v);
+    } else {
 #pragma unroll
-      for (int i = 0; i < N; i++) h[i] = from_float<O>(v[i]);
-      *reinterpret_cast<uint4*>(to) = a;
+      for (int i = 0; i < N; i++) v[i] = e + i < end ? to_float(from[e + i]) : 0.f;
+    }
+    if (DROP) {
+      const unsigned bits = kept[(e - e0) / 32] >> ((e - e0) & 31);
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = bits >> i & 1 ? v[i] * A.D.scale : 0.f;
+    }
+    if (whole) {
+      store_cols<O, N>(to + e, 0, N, v);
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++)
-        if (e + i < n) to[i] = from_float<O>(v[i]);
+        if (e + i < end) to[e + i] = from_float<O>(v[i]);
     }
   }
 }
@@ -223,7 +245,8 @@ __global__ void k_next_draw(unsigned long long* state, unsigned long long* taken
 template <bool LOOKUP>
 cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vectors* out, int width, float scale, const Drop& D, long* launches,
                         cudaStream_t st) {
-  RowArgs A = {S, 0, S.rows, width, FastDiv((unsigned)((long long)width + 7 >> 3)), FastDiv((unsigned)width), src->ld, out->ld, scale, D};
+  const unsigned eights = (unsigned)(((long long)width + 7) >> 3);
+  RowArgs A = {S, 0, S.rows, width, eights, 0, 0, FastDiv(eights), FastDiv((unsigned)width), FastDiv(), src->ld, out->ld, scale, D};
   const bool aligned = rows_aligned(src) && rows_aligned(out);
   const bool flat = out->ld == width && reinterpret_cast<uintptr_t>(out->data) % 16 == 0 &&
                     (LOOKUP || (src->ld == width && reinterpret_cast<uintptr_t>(src->data) % 16 == 0));
@@ -242,18 +265,27 @@ cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vector
     }
     for (A.first = 0; A.first < S.rows && e == cudaSuccess; A.first += A.rows) {
       A.rows = S.rows - A.first < most ? S.rows - A.first : most;
-      const unsigned units = A.rows * A.by_groups.d;
       ++*launches;
       if (!aligned) {
         e = launch_early(drops(D) ? k_rows_flat<T, O, LOOKUP, true> : k_rows_flat<T, O, LOOKUP, false>,
                          dim3((unsigned)(((long long)A.rows * width + FLAT - 1) / FLAT)), 256, 0, st, A, from, to);
-      } else if (units <= 148 * 256 * 4) {  // one wave: more threads instead of more units a thread
-        e = launch_early(drops(D) ? k_rows_aligned<T, O, LOOKUP, true, 1> : k_rows_aligned<T, O, LOOKUP, false, 1>, dim3((units + 255) / 256), 256, 0, st,
-                         A, from, to);
-      } else {
-        e = launch_early(drops(D) ? k_rows_aligned<T, O, LOOKUP, true, 4> : k_rows_aligned<T, O, LOOKUP, false, 4>, dim3((units + 1023) / 1024), 256, 0, st,
-                         A, from, to);
+        continue;
       }
+      // 16 bytes a thread of whatever is wider; dropout goes by eights
+      const bool fours = !drops(D) && (sizeof(T) == 4 || sizeof(O) == 4);
+      A.groups = fours ? (unsigned)(width + 3) / 4 : eights;
+      const unsigned tiles = (A.groups + 255) / 256;
+      A.across = (A.groups + tiles - 1) / tiles;
+      A.down = 256 / A.across;
+      A.by_across = FastDiv(A.across);
+      // few rows: more threads instead of more rows a thread
+      const int units = (size_t)A.rows * A.groups <= 148 * 512 ? 1 : drops(D) ? 2 : UNITS_MOST;
+      const dim3 grid((A.rows + A.down * units - 1) / (A.down * units), tiles);
+      const unsigned threads = (A.across * A.down + 31) / 32 * 32;
+      auto kernel = units == 1 ? k_rows_aligned<T, O, LOOKUP, true, 8, 1> : k_rows_aligned<T, O, LOOKUP, true, 8, 2>;
+      if (fours) kernel = units == 1 ? k_rows_aligned<T, O, LOOKUP, false, 4, 1> : k_rows_aligned<T, O, LOOKUP, false, 4, UNITS_MOST>;
+      else if (!drops(D)) kernel = units == 1 ? k_rows_aligned<T, O, LOOKUP, false, 8, 1> : k_rows_aligned<T, O, LOOKUP, false, 8, UNITS_MOST>;
+      e = launch_early(kernel, grid, threads, 0, st, A, from, to);
     }
     return e;
   });

@@ -12,79 +12,99 @@ namespace lmg {
 namespace {
 
 // ---- few types --------------------------------------------------------------------------------------------------------
-constexpr int TABLE_WARPS = 8, TABLE_COLS = 32, TABLE_ROWS = 8;  // rows whose loads are in flight together
+constexpr int TABLE_COLS = 32, TABLE_LANES = 8;  // columns of a table, lanes that share a row: four columns each
 
-// a warp takes `per` consecutive slots, a lane one of 32 columns; parts[block][type][width], or `grad` where one block does all
-template <class T, class O, bool DROP>
-__global__ void __launch_bounds__(TABLE_WARPS * 32) k_type_tables(Slots S, unsigned per, const T* diff, long long diff_ld, int width, float* parts,
-                                                                  O* grad, long long grad_ld, float scale, Drop D) {
-  extern __shared__ float tables[];  // [warp][type][32]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, V = S.ntypes;
-  for (int i = threadIdx.x; i < TABLE_WARPS * V * TABLE_COLS; i += blockDim.x) tables[i] = 0.f;
-  __syncthreads();
+// A warp takes 32 consecutive slots at a time, four side by side: eight lanes with a table of their own, which nobody else touches, add
+// them to it one after the other.  parts[block][type][width], or `grad` where one block does all.  (A lane a column and a
+// table a warp instead took 33 instructions a slot and 16 us for 200000 slots of 28.)
+template <class T, class O, bool VEC, bool DROP>
+__global__ void __launch_bounds__(512) k_type_tables(Slots S, unsigned per, const T* diff, long long diff_ld, int width, float* parts, O* grad,
+                                                     long long grad_ld, float scale, Drop D) {
+  extern __shared__ float4 tables[];  // [warp][4][type][8]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, warps = blockDim.x / 32, V = S.ntypes, q = lane / TABLE_LANES, l = lane % TABLE_LANES;
+  for (int i = threadIdx.x; i < warps * 4 * V * TABLE_LANES; i += blockDim.x) tables[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   wait_for_stream();
   const DropKey K(D);
-  float* mine = tables + warp * V * TABLE_COLS + lane;
-  const int col = blockIdx.y * TABLE_COLS + lane;
-  const unsigned begin = min((unsigned long long)(blockIdx.x * TABLE_WARPS + warp) * per, (unsigned long long)S.rows);
-  const unsigned end = min((unsigned long long)begin + per, (unsigned long long)S.rows);
+  float4* mine = tables + (size_t)(warp * 4 + q) * V * TABLE_LANES + l;
+  const int col = blockIdx.y * TABLE_COLS + l * 4;
+  const unsigned long long at = (unsigned long long)(blockIdx.x * warps + warp) * per;
+  const unsigned begin = at < S.rows ? (unsigned)at : S.rows, end = S.rows - begin < per ? S.rows : begin + per;
+  // types two turns ahead, values one
+  auto types = [&](unsigned r0) { return r0 < end && end - r0 > lane ? slot_type(S, r0 + lane) : -1; };
+  int t[8], t_next[8];
+  Raw<T, 4, VEC> raw[8], raw_next[8];
+  auto fetch = [&](unsigned r0, int type, int (&to_t)[8], Raw<T, 4, VEC> (&to_v)[8]) {
+    const T* from = diff + (long long)(r0 + q) * diff_ld;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      to_t[j] = __shfl_sync(0xffffffffu, type, j * 4 + q);
+      if (col >= width) to_t[j] = -1;
+      if (to_t[j] >= 0) to_v[j].load(from + j * 4 * diff_ld, col, width);
+    }
+  };
+  fetch(begin, types(begin), t, raw);
+  int type_next = types(begin + 32);
+  __syncthreads();
   for (unsigned r0 = begin; r0 < end; r0 += 32) {
-    const int type = r0 + lane < end ? slot_type(S, r0 + lane) : -1;
-    const T* from = diff + (long long)r0 * diff_ld + col;
+    fetch(r0 + 32, type_next, t_next, raw_next);
+    type_next = types(r0 + 64);
+    unsigned keep[8];
+    if (DROP) {
+      // eight slots of four groups of eight columns a turn: a lane draws for one of them and hands its bits round
 #pragma unroll
-    for (int j0 = 0; j0 < 32; j0 += TABLE_ROWS) {
-      if (r0 + j0 >= end) break;
-      float v[TABLE_ROWS];
-      int t[TABLE_ROWS];
+      for (int j = 0; j < 8; j += 2) {
+        const unsigned bits = kept8(D, K, r0 + j * 4 + lane / 4, blockIdx.y * (TABLE_COLS / 8) + lane % 4);
 #pragma unroll
-      for (int j = 0; j < TABLE_ROWS; j++) {
-        t[j] = __shfl_sync(0xffffffffu, type, j0 + j);
-        v[j] = t[j] >= 0 && col < width ? to_float(from[(j0 + j) * diff_ld]) : 0.f;
+        for (int h = 0; h < 2; h++) keep[j + h] = __shfl_sync(0xffffffffu, bits, (h * 4 + q) * 4 + l / 2) >> (l & 1) * 4;
       }
-      if (DROP) {
-        // 8 rows of 4 groups of 8 columns: a lane draws for one of them and hands its bits round
-        const unsigned bits = kept8(D, K, r0 + j0 + lane / 4, blockIdx.y * (TABLE_COLS / 8) + lane % 4);
+    }
 #pragma unroll
-        for (int j = 0; j < TABLE_ROWS; j++) {
-          const unsigned b = __shfl_sync(0xffffffffu, bits, j * 4 + lane / 8);
-          v[j] = b >> (lane & 7) & 1 ? v[j] * D.scale : 0.f;
-        }
+    for (int j = 0; j < 8; j++) {
+      if (t[j] >= 0) {
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = DROP ? (keep[j] >> c & 1 ? raw[j].get(c) * D.scale : 0.f) : raw[j].get(c);
+        float4* to = mine + t[j] * TABLE_LANES;
+        float4 s = *to;
+        s.x += v[0], s.y += v[1], s.z += v[2], s.w += v[3];
+        *to = s;
       }
-#pragma unroll
-      for (int j = 0; j < TABLE_ROWS; j++)
-        if (t[j] >= 0) mine[t[j] * TABLE_COLS] += v[j];
+      t[j] = t_next[j];
+      raw[j] = raw_next[j];
     }
   }
   __syncthreads();
+  const float* all = reinterpret_cast<const float*>(tables);
   for (int i = threadIdx.x; i < V * TABLE_COLS; i += blockDim.x) {
-    const int c = blockIdx.y * TABLE_COLS + (i & (TABLE_COLS - 1)), t = i / TABLE_COLS;
+    const int c = blockIdx.y * TABLE_COLS + (i & (TABLE_COLS - 1)), type = i / TABLE_COLS;
     if (c >= width) continue;
     float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < TABLE_WARPS; w++) sum += tables[w * V * TABLE_COLS + i];
-    if (gridDim.x == 1) grad[(long long)t * grad_ld + c] = from_float<O>(sum * scale);
-    else parts[((size_t)blockIdx.x * V + t) * width + c] = sum;
+#pragma unroll 8
+    for (int w = 0; w < warps * 4; w++) sum += all[(size_t)w * V * TABLE_COLS + i];
+    if (gridDim.x == 1) grad[(long long)type * grad_ld + c] = from_float<O>(sum * scale);
+    else parts[((size_t)blockIdx.x * V + type) * width + c] = sum;
   }
 }
 
-// the sum of all blocks' tables: 32 values a block, eight threads a value
+// the sum of all blocks' tables: 32 values a block, 32 threads a value
 template <class O>
-__global__ void __launch_bounds__(256) k_table_sums(const float* parts, int n, int V, int width, O* grad, long long grad_ld, float scale) {
-  __shared__ float s[8][32];
+__global__ void __launch_bounds__(1024) k_table_sums(const float* parts, int n, int V, int width, O* grad, long long grad_ld, float scale) {
+  __shared__ float s[32][33];
   wait_for_stream();
-  const size_t M = (size_t)V * width, o = (size_t)blockIdx.x * 32 + threadIdx.x % 32;
-  const int slice = threadIdx.x / 32;
+  const size_t M = (size_t)V * width, first = (size_t)blockIdx.x * 32;
+  const int lane = threadIdx.x & 31, slice = threadIdx.x / 32;
   float sum = 0.f;
-  if (o < M) {
+  if (first + lane < M) {
 #pragma unroll 8
-    for (int p = slice; p < n; p += 8) sum += parts[p * M + o];
+    for (int p = slice; p < n; p += 32) sum += parts[p * M + first + lane];
   }
-  s[slice][threadIdx.x % 32] = sum;
+  s[slice][lane] = sum;
   __syncthreads();
-  if (slice == 0 && o < M) {
-    for (int i = 1; i < 8; i++) sum += s[i][threadIdx.x];
-    grad[(long long)(o / width) * grad_ld + o % width] = from_float<O>(sum * scale);
-  }
+  sum = s[lane][slice];  // a warp a value
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const size_t o = first + slice;
+  if (lane == 0 && o < M) grad[(long long)(o / width) * grad_ld + o % width] = from_float<O>(sum * scale);
 }
 
 // ---- the sort ---------------------------------------------------------------------------------------------------------
@@ -215,100 +235,145 @@ size_t sort_smem(int bits) {
 // ---- sums of sorted slots ---------------------------------------------------------------------------------------------
 struct PieceArgs {
   const unsigned *key, *row;
-  unsigned n, ntypes, piece, pieces;
-  int lanes;     // that share a piece, eight columns each; a power of two
+  unsigned n, ntypes, piece;
+  int lanes;        // that share a piece, eight columns each; a power of two
+  unsigned blocks;  // of PIECE_THREADS / lanes pieces
   int width;
-  float* parts;  // [pieces][2][width]: of the type that comes in from the piece before, of the one that goes on in the next
+  float* parts;     // [blocks][2][width]: of the type that comes in from the block before, of the one that goes on in the next
   float scale;
 };
 
-constexpr int PIECE_THREADS = 256, PIECE_ROWS = 4;
+constexpr int PIECE_THREADS = 256, PIECE_SLOTS = 2048;  // slots of a block, at most
 
+// A group of lanes sums a piece type by type.  A type that crosses pieces is put together in shared memory by the group that it begins
+// in; only what crosses blocks is left to k_type_joins (one of a hundred pieces, so the way of a type that holds
+// many slots is short: 46 us for 25000 slots, a tenth of them of one type, without).
 template <class T, class O, bool VEC, bool DROP>
-__global__ void __launch_bounds__(PIECE_THREADS) k_type_pieces(PieceArgs A, const T* diff, long long diff_ld, O* grad, long long grad_ld, Drop D) {
+__global__ void __launch_bounds__(PIECE_THREADS, 3) k_type_pieces(PieceArgs A, const T* diff, long long diff_ld, O* grad, long long grad_ld, Drop D) {
+  constexpr int ROWS = sizeof(T) == 2 ? 8 : 4;  // whose loads are in flight together
+  __shared__ unsigned keys[PIECE_SLOTS + 2], rows[PIECE_SLOTS];
+  __shared__ float heads[PIECE_THREADS * 8], tails[PIECE_THREADS * 8];
   wait_for_stream();
-  const unsigned at = blockIdx.x * PIECE_THREADS + threadIdx.x, piece = at / A.lanes;
-  const int col = (blockIdx.y * A.lanes + at % A.lanes) * 8;
-  if (piece >= A.pieces || col >= A.width) return;
-  const DropKey K(D);
-  const unsigned begin = piece * A.piece, end = min(begin + A.piece, A.n);
-  const unsigned came = begin > 0 ? A.key[begin - 1] : ~0u, goes = end < A.n ? A.key[end] : ~0u;
-  float sum[8] = {};
-  unsigned type = A.key[begin];
-  bool first = true;
-  auto put = [&](bool last) {
-    if (type >= A.ntypes) return;
-    if (first && type == came) {
-      store8<float, false>(A.parts + (size_t)piece * 2 * A.width, col, A.width, sum);
-    } else if (last && type == goes) {
-      store8<float, false>(A.parts + ((size_t)piece * 2 + 1) * A.width, col, A.width, sum);
-    } else {
+  const int groups = PIECE_THREADS / A.lanes, group = threadIdx.x / A.lanes, lane = threadIdx.x % A.lanes;
+  const unsigned slots = groups * A.piece, first_slot = blockIdx.x * slots, here = min(slots, A.n - first_slot);
+  for (unsigned i = threadIdx.x; i < here + 2; i += PIECE_THREADS) {
+    const unsigned at = first_slot + i;  // keys[i] is that of the slot before
+    keys[i] = at > 0 && at <= A.n ? A.key[at - 1] : ~0u;
+    if (i < here) rows[i] = A.row[at];
+  }
+  __syncthreads();
+  const int col = (blockIdx.y * A.lanes + lane) * 8;
+  const unsigned begin = min(group * A.piece, here), end = min(begin + A.piece, here);
+  const bool some = begin < end && col < A.width;
+  const unsigned came = keys[begin], goes = keys[end + 1];
+  float* head = heads + (size_t)group * A.lanes * 8 + lane * 8;
+  float* tail = tails + (size_t)group * A.lanes * 8 + lane * 8;
+  auto write = [&](unsigned type, float (&sum)[8]) {
 #pragma unroll
-      for (int c = 0; c < 8; c++) sum[c] *= A.scale;
-      store8<O, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
+    for (int c = 0; c < 8; c++) sum[c] *= A.scale;
+    store_cols<O, 8, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
+  };
+  if (some) {
+    const DropKey K(D);
+    float sum[8] = {};
+    unsigned type = keys[begin + 1];
+    bool first = true;
+    auto put = [&](bool last) {
+      if (type >= A.ntypes) return;
+      if (first && type == came) {
+#pragma unroll
+        for (int c = 0; c < 8; c++) head[c] = sum[c];
+      } else if (last && type == goes) {
+#pragma unroll
+        for (int c = 0; c < 8; c++) tail[c] = sum[c];
+      } else {
+        write(type, sum);
+      }
+    };
+    for (unsigned i = begin; i < end; i += ROWS) {
+      Raw<T, 8, VEC> v[ROWS];
+#pragma unroll
+      for (int j = 0; j < ROWS; j++)
+        if (i + j < end && keys[i + j + 1] < A.ntypes) v[j].load(diff + (long long)rows[i + j] * diff_ld, col, A.width);
+#pragma unroll
+      for (int j = 0; j < ROWS; j++) {
+        if (i + j >= end) break;
+        const unsigned t = keys[i + j + 1];
+        if (t != type) {
+          put(false);
+          first = false;
+          type = t;
+#pragma unroll
+          for (int c = 0; c < 8; c++) sum[c] = 0.f;
+        }
+        if (type >= A.ntypes) continue;
+        const unsigned keep = DROP ? kept8(D, K, rows[i + j], col / 8) : 0xff;
+#pragma unroll
+        for (int c = 0; c < 8; c++) sum[c] += DROP ? (keep >> c & 1 ? v[j].get(c) * D.scale : 0.f) : v[j].get(c);
+      }
+    }
+    put(true);
+  }
+  __syncthreads();
+  if (!some) return;
+  // the heads of pieces from `p` on, while the type goes on; true: beyond the block
+  auto follow = [&](unsigned type, unsigned p, float (&sum)[8]) {
+    for (;; p++) {
+      if (p * A.piece >= here) return true;
+      const float* h = heads + (size_t)p * A.lanes * 8 + lane * 8;
+#pragma unroll
+      for (int c = 0; c < 8; c++) sum[c] += h[c];
+      const unsigned last = min((p + 1) * A.piece, here);
+      if (keys[last] != type || keys[last + 1] != type) return false;
     }
   };
-  for (unsigned i = begin; i < end; i += PIECE_ROWS) {
-    unsigned t[PIECE_ROWS], r[PIECE_ROWS];
-    float v[PIECE_ROWS][8];
-#pragma unroll
-    for (int j = 0; j < PIECE_ROWS; j++) {
-      t[j] = i + j < end ? A.key[i + j] : A.ntypes;
-      r[j] = i + j < end ? A.row[i + j] : 0;
-    }
-#pragma unroll
-    for (int j = 0; j < PIECE_ROWS; j++)
-      if (t[j] < A.ntypes) load8<T, VEC>(diff + (long long)r[j] * diff_ld, col, A.width, v[j]);
-#pragma unroll
-    for (int j = 0; j < PIECE_ROWS; j++) {
-      if (i + j >= end) break;
-      if (t[j] != type) {
-        put(false);
-        first = false;
-        type = t[j];
-#pragma unroll
-        for (int c = 0; c < 8; c++) sum[c] = 0.f;
-      }
-      if (type >= A.ntypes) continue;
-      const unsigned keep = DROP ? kept8(D, K, r[j], col / 8) : 0xff;
-#pragma unroll
-      for (int c = 0; c < 8; c++) sum[c] += DROP ? (keep >> c & 1 ? v[j][c] * D.scale : 0.f) : v[j][c];
-    }
+  float* parts = A.parts + (size_t)blockIdx.x * 2 * A.width;
+  const unsigned t0 = keys[begin + 1], t1 = keys[end];
+  if (group == 0 && t0 == came && t0 < A.ntypes) {
+    float sum[8] = {};
+    follow(t0, 0, sum);
+    store_cols<float, 8, false>(parts, col, A.width, sum);
   }
-  put(true);
+  if (goes == t1 && t1 < A.ntypes && !(t0 == t1 && came == t0)) {
+    float sum[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) sum[c] = tail[c];
+    if (follow(t1, group + 1, sum)) store_cols<float, 8, false>(parts + A.width, col, A.width, sum);
+    else write(t1, sum);
+  }
 }
 
-// a type that begins in a piece and goes on: its parts, piece after piece
+// a type that begins in a block and goes on: its parts, block after block
 template <class O, bool VEC>
 __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* grad, long long grad_ld) {
   wait_for_stream();
-  const unsigned at = blockIdx.x * PIECE_THREADS + threadIdx.x, piece = at / A.lanes;
+  const unsigned at = blockIdx.x * PIECE_THREADS + threadIdx.x, block = at / A.lanes, slots = PIECE_THREADS / A.lanes * A.piece;
   const int col = (blockIdx.y * A.lanes + at % A.lanes) * 8;
-  if (piece + 1 >= A.pieces || col >= A.width) return;
-  const unsigned begin = piece * A.piece, end = begin + A.piece, type = A.key[end - 1];
+  if (block + 1 >= A.blocks || col >= A.width) return;
+  const unsigned begin = block * slots, end = begin + slots, type = A.key[end - 1];
   if (type >= A.ntypes || A.key[end] != type || (begin > 0 && A.key[begin - 1] == type)) return;
   float sum[8];
-  load8<float, false>(A.parts + ((size_t)piece * 2 + 1) * A.width, col, A.width, sum);
-  unsigned p = piece + 1;
-  while (p + 4 <= A.pieces && A.key[(p + 3) * A.piece] == type) {
+  load_cols<float, 8, false>(A.parts + ((size_t)block * 2 + 1) * A.width, col, A.width, sum);
+  unsigned p = block + 1;
+  while (p + 4 <= A.blocks && A.key[(p + 3) * slots] == type) {
     float v[4][8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) load8<float, false>(A.parts + (size_t)(p + j) * 2 * A.width, col, A.width, v[j]);
+    for (int j = 0; j < 4; j++) load_cols<float, 8, false>(A.parts + (size_t)(p + j) * 2 * A.width, col, A.width, v[j]);
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
       for (int c = 0; c < 8; c++) sum[c] += v[j][c];
     p += 4;
   }
-  for (; p < A.pieces && A.key[p * A.piece] == type; p++) {
+  for (; p < A.blocks && A.key[p * slots] == type; p++) {
     float v[8];
-    load8<float, false>(A.parts + (size_t)p * 2 * A.width, col, A.width, v);
+    load_cols<float, 8, false>(A.parts + (size_t)p * 2 * A.width, col, A.width, v);
 #pragma unroll
     for (int c = 0; c < 8; c++) sum[c] += v[c];
   }
 #pragma unroll
   for (int c = 0; c < 8; c++) sum[c] *= A.scale;
-  store8<O, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
+  store_cols<O, 8, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
 }
 
 // ---- the plan: a function of the sizes alone, so that the workspace and the call agree ----------------------------------------
@@ -316,39 +381,39 @@ struct Plan {
   bool tables;
   // few types
   unsigned blocks, per;
+  int warps;
   size_t table_smem;
   // sorted
   unsigned tiles, tile;
   int passes, bits;
-  unsigned piece, pieces;
+  unsigned piece, piece_blocks;
   int lanes;
   size_t key[2], row[2], counts, parts, bytes;
 };
 
-constexpr size_t TABLE_SMEM_MOST = 200 << 10;
+constexpr size_t TABLE_SMEM = 224 << 10;  // an SM's
+constexpr int TABLE_WARPS_LEAST = 4, TABLE_WARPS_MOST = 16;
 
 Plan plan_for(unsigned rows, int V, int width) {
   Plan p = {};
-  const unsigned col_tiles = (width + TABLE_COLS - 1) / TABLE_COLS;
-  p.table_smem = (size_t)TABLE_WARPS * V * TABLE_COLS * 4;
   if (V == 0 || width == 0 || rows == 0) {
-    p.tables = true;
-    p.blocks = 1;
-    p.per = 32;
     p.bytes = 256;
     return p;
   }
-  if (p.table_smem <= TABLE_SMEM_MOST) {
-    const unsigned resident = 148 * (unsigned)(p.table_smem * 8 <= 220 << 10 ? 8 : (220 << 10) / (p.table_smem + 1024));
-    unsigned blocks = resident / col_tiles > 0 ? resident / col_tiles : 1;
-    const unsigned most = (rows + TABLE_WARPS * 32 - 1) / (TABLE_WARPS * 32);  // 32 slots a warp
-    if (blocks > most) blocks = most;
+  // tables: four a warp; fewer than four warps an SM have too few loads in flight
+  const size_t warp_smem = (size_t)4 * V * TABLE_COLS * 4;
+  if (warp_smem * TABLE_WARPS_LEAST <= TABLE_SMEM) {
+    p.warps = (int)(TABLE_SMEM / warp_smem < TABLE_WARPS_MOST ? TABLE_SMEM / warp_smem : TABLE_WARPS_MOST);
+    const unsigned all = (rows + 31) / 32;  // warps that find 32 slots
+    if (all < 148u * p.warps) p.warps = all / 148 < TABLE_WARPS_LEAST ? TABLE_WARPS_LEAST : (int)(all / 148);
+    p.blocks = (all + p.warps - 1) / p.warps < 148 ? (all + p.warps - 1) / p.warps : 148;
     // the blocks' tables are written and read once more: worth it while they are a fraction of the gradients
-    if ((size_t)blocks * V <= rows || blocks == 1) {
+    if ((size_t)p.blocks * V <= rows || p.blocks == 1) {
       p.tables = true;
-      const unsigned warps = blocks * TABLE_WARPS;
+      p.table_smem = warp_smem * p.warps;
+      const unsigned warps = p.blocks * p.warps;
       p.per = ((rows + warps - 1) / warps + 31) / 32 * 32;
-      p.blocks = (rows + p.per * TABLE_WARPS - 1) / (p.per * TABLE_WARPS);
+      p.blocks = (unsigned)(((unsigned long long)rows + (unsigned long long)p.per * p.warps - 1) / ((unsigned long long)p.per * p.warps));
       p.bytes = 256 + (size_t)p.blocks * V * width * 4;
       return p;
     }
@@ -365,11 +430,12 @@ Plan plan_for(unsigned rows, int V, int width) {
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes * 8 < width) p.lanes *= 2;
   const unsigned cols = (width + p.lanes * 8 - 1) / (p.lanes * 8);
-  // pieces for 32 warps an SM, of 8 to 256 slots
-  const size_t want = (size_t)rows * cols * p.lanes / (148 * 32 * 32);
+  // pieces for 64 warps an SM, of 8 to 32 slots
+  const size_t want = (size_t)rows * cols * p.lanes / (148 * 64 * 32);
   p.piece = 8;
-  while (p.piece < 256 && p.piece < want) p.piece *= 2;
-  p.pieces = (rows + p.piece - 1) / p.piece;
+  while (p.piece < 32 && p.piece < want && p.piece * 2 * (PIECE_THREADS / p.lanes) <= PIECE_SLOTS) p.piece *= 2;
+  const unsigned slots = p.piece * (PIECE_THREADS / p.lanes);
+  p.piece_blocks = (rows + slots - 1) / slots;
   size_t at = 256;
   for (int k = 0; k < 2; k++) {
     p.key[k] = at;
@@ -380,7 +446,7 @@ Plan plan_for(unsigned rows, int V, int width) {
   p.counts = at;
   at += aligned256(((size_t)p.tiles << p.bits) * 4);
   p.parts = at;
-  at += (size_t)p.pieces * 2 * width * 4;
+  at += (size_t)p.piece_blocks * 2 * width * 4;
   p.bytes = at;
   return p;
 }
@@ -397,16 +463,18 @@ cudaError_t by_tables(const Slots& S, const Plan& p, const lmg_vectors* diff, co
                       char* ws, long* launches, cudaStream_t st) {
   float* parts = reinterpret_cast<float*>(ws + 256);
   O* g = static_cast<O*>(grad->data);
-  const auto kernel = drops(D) ? k_type_tables<T, O, true> : k_type_tables<T, O, false>;
+  const bool vec = rows_aligned(diff);
+  const auto kernel = vec ? (drops(D) ? k_type_tables<T, O, true, true> : k_type_tables<T, O, true, false>)
+                          : (drops(D) ? k_type_tables<T, O, false, true> : k_type_tables<T, O, false, false>);
   cudaError_t e = allow_smem(kernel, p.table_smem);
   if (e == cudaSuccess)
-    e = launch_early(kernel, dim3(p.blocks, (width + TABLE_COLS - 1) / TABLE_COLS), TABLE_WARPS * 32, p.table_smem, st, S, p.per,
+    e = launch_early(kernel, dim3(p.blocks, (width + TABLE_COLS - 1) / TABLE_COLS), 32 * p.warps, p.table_smem, st, S, p.per,
                      static_cast<const T*>(diff->data), diff->ld, width, parts, g, grad->ld, scale, D);
   if (e != cudaSuccess) return e;
   ++*launches;
   if (p.blocks == 1) return e;
   ++*launches;
-  return launch_early(k_table_sums<O>, dim3((unsigned)(((size_t)S.ntypes * width + 31) / 32)), 256, 0, st, parts, (int)p.blocks, S.ntypes, width, g,
+  return launch_early(k_table_sums<O>, dim3((unsigned)(((size_t)S.ntypes * width + 31) / 32)), 1024, 0, st, parts, (int)p.blocks, S.ntypes, width, g,
                       grad->ld, scale);
 }
 
@@ -456,20 +524,21 @@ cudaError_t by_sort(const Slots& S, const Plan& p, const lmg_vectors* diff, cons
   P.n = S.rows;
   P.ntypes = (unsigned)S.ntypes;
   P.piece = p.piece;
-  P.pieces = p.pieces;
+  P.blocks = p.piece_blocks;
   P.lanes = p.lanes;
   P.width = width;
   P.parts = reinterpret_cast<float*>(ws + p.parts);
   P.scale = scale;
   const bool vec = rows_aligned(diff) && rows_aligned(grad);
-  const dim3 grid((unsigned)(((size_t)p.pieces * p.lanes + PIECE_THREADS - 1) / PIECE_THREADS), (width + p.lanes * 8 - 1) / (p.lanes * 8));
+  const unsigned cols = (width + p.lanes * 8 - 1) / (p.lanes * 8);
   const auto pieces = vec ? (drops(D) ? k_type_pieces<T, O, true, true> : k_type_pieces<T, O, true, false>)
                           : (drops(D) ? k_type_pieces<T, O, false, true> : k_type_pieces<T, O, false, false>);
-  e = launch_early(pieces, grid, PIECE_THREADS, 0, st, P, static_cast<const T*>(diff->data), diff->ld, static_cast<O*>(grad->data), grad->ld, D);
+  e = launch_early(pieces, dim3(p.piece_blocks, cols), PIECE_THREADS, 0, st, P, static_cast<const T*>(diff->data), diff->ld, static_cast<O*>(grad->data), grad->ld, D);
   if (e != cudaSuccess) return e;
   ++*launches;
-  if (p.pieces == 1) return e;
+  if (p.piece_blocks == 1) return e;
   ++*launches;
+  const dim3 grid((unsigned)(((size_t)p.piece_blocks * p.lanes + PIECE_THREADS - 1) / PIECE_THREADS), cols);
   return launch_early(vec ? k_type_joins<O, true> : k_type_joins<O, false>, grid, PIECE_THREADS, 0, st, P, static_cast<O*>(grad->data), grad->ld);
 }
 

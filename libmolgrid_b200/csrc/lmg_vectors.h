@@ -40,8 +40,8 @@ struct Slots {
 };
 
 struct Drop {
-  unsigned threshold_hi, threshold_lo;  // upper half (up to 65536) and lower half of p * 2^32
-  float scale;                          // 1 / (1 - p)
+  unsigned upper, lower;  // p * 2^32 = upper * 65536 + lower; 2^32 itself as 65535 and 65536
+  float scale;            // 1 / (1 - p)
   unsigned long long seed, offset;
   const unsigned long long* state;
 };
@@ -53,15 +53,17 @@ __device__ __forceinline__ bool slot_filled(const Slots& S, unsigned row) {
   return (int)(row - b * S.n) < S.n_atoms[b];
 }
 
-// type of a slot, -1 where it is empty
+// type of a slot, -1 where it is empty; its count and its index are on their way together
 __device__ __forceinline__ int slot_type(const Slots& S, unsigned row) {
-  if (!slot_filled(S, row)) return -1;
-  bool high;
+  bool filled = true, high;
   int t;
+  if (S.n_atoms != nullptr) {
+    const unsigned b = S.by_n(row);
+    filled = (int)(row - b * S.n) < S.n_atoms[b];
+  }
   if (S.index_type == LMG_INDEX_FLOAT32) {
     const float f = roundf(static_cast<const float*>(S.index)[row]);
-    if (!(f >= 0.f)) return -1;
-    t = f < 2147483648.f ? (int)f : 0x7fffffff;
+    t = f >= 0.f ? f < 2147483648.f ? (int)f : 0x7fffffff : -1;
     high = t >= S.ntypes;
   } else if (S.index_type == LMG_INDEX_INT32) {
     t = static_cast<const int*>(S.index)[row];
@@ -71,11 +73,8 @@ __device__ __forceinline__ int slot_type(const Slots& S, unsigned row) {
     high = l >= S.ntypes;
     t = l < 0 ? -1 : (int)l;
   }
-  if (high) {
-    if (S.status != nullptr) *S.status = 1;
-    return -1;
-  }
-  return t < 0 ? -1 : t;
+  if (filled && high && S.status != nullptr) *S.status = 1;
+  return filled && !high && t >= 0 ? t : -1;
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -86,14 +85,19 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// eight values of a row from column `col` on, zeros behind its end; VEC: column 0 lies on 16 bytes and `col` is a multiple of 8
-template <class T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int col, int width, float (&v)[8]) {
-  constexpr int N = VEC ? 16 / sizeof(T) : 8;
+template <int N> struct Bytes;
+template <> struct Bytes<16> { typedef uint4 type; };
+template <> struct Bytes<8> { typedef uint2 type; };
+
+// COLS values of a row from column `col` on, a multiple of COLS, zeros behind its end; VEC: the row begins on 16 bytes, and they are
+// read 16 bytes at a time, or as many as they are
+template <class T, int COLS, bool VEC = true>
+__device__ __forceinline__ void load_cols(const T* row, int col, int width, float (&v)[COLS]) {
+  constexpr int N = !VEC ? COLS : COLS * sizeof(T) < 16 ? COLS : 16 / sizeof(T);
 #pragma unroll
-  for (int k = 0; k < 8; k += N) {
+  for (int k = 0; k < COLS; k += N) {
     if (VEC && col + k + N <= width) {
-      const uint4 a = *reinterpret_cast<const uint4*>(row + col + k);
+      typename Bytes<VEC ? N * sizeof(T) : 16>::type a = *reinterpret_cast<const typename Bytes<VEC ? N * sizeof(T) : 16>::type*>(row + col + k);
       const T* e = reinterpret_cast<const T*>(&a);
 #pragma unroll
       for (int i = 0; i < N; i++) v[k + i] = to_float(e[i]);
@@ -104,17 +108,17 @@ __device__ __forceinline__ void load8(const T* row, int col, int width, float (&
   }
 }
 
-template <class T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int col, int width, const float (&v)[8]) {
-  constexpr int N = VEC ? 16 / sizeof(T) : 8;
+template <class T, int COLS, bool VEC = true>
+__device__ __forceinline__ void store_cols(T* row, int col, int width, const float (&v)[COLS]) {
+  constexpr int N = !VEC ? COLS : COLS * sizeof(T) < 16 ? COLS : 16 / sizeof(T);
 #pragma unroll
-  for (int k = 0; k < 8; k += N) {
+  for (int k = 0; k < COLS; k += N) {
     if (VEC && col + k + N <= width) {
-      uint4 a;
+      typename Bytes<VEC ? N * sizeof(T) : 16>::type a;
       T* e = reinterpret_cast<T*>(&a);
 #pragma unroll
       for (int i = 0; i < N; i++) e[i] = from_float<T>(v[k + i]);
-      *reinterpret_cast<uint4*>(row + col + k) = a;
+      *reinterpret_cast<typename Bytes<VEC ? N * sizeof(T) : 16>::type*>(row + col + k) = a;
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++)
@@ -123,16 +127,60 @@ __device__ __forceinline__ void store8(T* row, int col, int width, const float (
   }
 }
 
-// Philox4x32-10: ten rounds of two 32 x 32 -> 64 bit products (Salmon, Moraes, Dror and Shaw, 2011, section 4.3)
-__device__ __forceinline__ uint4 philox(uint4 c, unsigned k0, unsigned k1) {
+// COLS values of a row as they lie, read long before they are used: half the registers for 16 bits
+template <class T, int COLS, bool VEC = true>
+struct Raw {
+  static constexpr int WORDS = COLS * sizeof(T) / 4;
+  unsigned w[WORDS];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const T* row, int col, int width) {
+    constexpr int N = !VEC ? COLS : WORDS < 4 ? COLS : 16 / (int)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < COLS; k += N) {
+      unsigned* to = w + k * sizeof(T) / 4;
+      if (VEC && col + k + N <= width) {
+        if constexpr (N * sizeof(T) == 16) {
+          const uint4 a = *reinterpret_cast<const uint4*>(row + col + k);
+          to[0] = a.x, to[1] = a.y, to[2] = a.z, to[3] = a.w;
+        } else {
+          const uint2 a = *reinterpret_cast<const uint2*>(row + col + k);
+          to[0] = a.x, to[1] = a.y;
+        }
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i++) to[i] = col + k + i < width ? __float_as_uint(row[col + k + i]) : 0u;
+      } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+        for (int i = 0; i < N; i += 2)
+          to[i / 2] = (col + k + i < width ? h[col + k + i] : 0u) | (col + k + i + 1 < width ? (unsigned)h[col + k + i + 1] << 16 : 0u);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    const unsigned short h = (unsigned short)(i & 1 ? w[i / 2] >> 16 : w[i / 2]);
+    return to_float(*reinterpret_cast<const T*>(&h));
+  }
+};
+
+// Philox4x32-10: ten rounds of two 32 x 32 -> 64 bit products (Salmon, Moraes, Dror and Shaw, 2011, section 4.3), N blocks side by
+// side under one key
+template <int N>
+__device__ __forceinline__ void philox(uint4 (&c)[N], unsigned k0, unsigned k1) {
 #pragma unroll
   for (int i = 0; i < 10; i++) {
-    const unsigned long long a = (unsigned long long)c.x * 0xD2511F53u, b = (unsigned long long)c.z * 0xCD9E8D57u;
-    c = make_uint4((unsigned)(b >> 32) ^ c.y ^ k0, (unsigned)b, (unsigned)(a >> 32) ^ c.w ^ k1, (unsigned)a);
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const unsigned long long a = (unsigned long long)c[j].x * 0xD2511F53u, b = (unsigned long long)c[j].z * 0xCD9E8D57u;
+      c[j] = make_uint4((unsigned)(b >> 32) ^ c[j].y ^ k0, (unsigned)b, (unsigned)(a >> 32) ^ c[j].w ^ k1, (unsigned)a);
+    }
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return c;
 }
 
 // key and offset of a call, read once a thread
@@ -147,29 +195,65 @@ struct DropKey {
   }
 };
 
-// which of the eight columns of a group stay, a bit each.  Sixteen bits a column decide all but a tie with the
-// threshold's upper half (one group in 8192); then the lower half is drawn too.
-__device__ __forceinline__ unsigned kept8(const Drop& D, const DropKey& K, unsigned row, unsigned group) {
-  const uint4 c = make_uint4(group, row, K.o0, K.o1);
-  const uint4 w = philox(c, K.k0, K.k1);
-  const unsigned word[4] = {w.x, w.y, w.z, w.w};
-  unsigned keep = 0, tie = 0;
+// A block's 128 bits decide eight columns, a half word each, but for a tie with the threshold's upper half (one block in 8192), for
+// which as many bits are drawn again: a bit for each column that loses its tie.  Apart, so that what calls it keeps its registers.
+static __device__ __noinline__ unsigned lost_ties(uint4 w, unsigned upper, unsigned lower, uint4 counter, unsigned k0, unsigned k1) {
+  uint4 v[1] = {make_uint4(counter.x, counter.y, counter.z, counter.w | 0x80000000u)};
+  philox(v, k0, k1);
+  const unsigned word[4] = {w.x, w.y, w.z, w.w}, low[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+  unsigned lost = 0;
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const unsigned h = j & 1 ? word[j / 2] >> 16 : word[j / 2] & 0xffffu;
-    keep |= (unsigned)(h >= D.threshold_hi) << j;
-    tie |= (unsigned)(h == D.threshold_hi) << j;
+    const int shift = j & 1 ? 16 : 0;
+    if ((word[j / 2] >> shift & 0xffffu) == upper && (low[j / 2] >> shift & 0xffffu) < lower) lost |= 1u << j;
   }
-  if (tie != 0 && D.threshold_lo != 0) {
-    const uint4 v = philox(make_uint4(c.x, c.y, c.z, c.w | 0x80000000u), K.k0, K.k1);
-    const unsigned low[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const unsigned h = j & 1 ? low[j / 2] >> 16 : low[j / 2] & 0xffffu;
-      if ((tie >> j & 1) && h < D.threshold_lo) keep &= ~(1u << j);
+  return lost;
+}
+
+// Which columns of a group stay.  Half words are compared where they are: the upper one of a word as the word, the lower one shifted up.
+struct Bits8 {
+  uint4 w;
+  unsigned least, lost;
+  __device__ __forceinline__ void set(uint4 words, const Drop& D, const DropKey& K, unsigned row, unsigned group) {
+    w = words;
+    least = D.upper << 16;
+    lost = 0;
+    if (D.lower != 0) {
+      const unsigned both = least | D.upper;
+      // the top bit of a half word is set if it, or one below it, equals the threshold
+      const unsigned x = w.x ^ both, y = w.y ^ both, z = w.z ^ both, u = w.w ^ both;
+      if ((((x - 0x00010001u) & ~x) | ((y - 0x00010001u) & ~y) | ((z - 0x00010001u) & ~z) | ((u - 0x00010001u) & ~u)) & 0x80008000u)
+        lost = lost_ties(w, D.upper, D.lower, make_uint4(group, row, K.o0, K.o1), K.k0, K.k1);
     }
   }
-  return keep;
+  __device__ __forceinline__ bool reaches(int j) const {
+    const unsigned v = j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w;
+    return (j & 1 ? v : v << 16) >= least;
+  }
+  __device__ __forceinline__ unsigned mask() const {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) m |= (unsigned)reaches(j) << j;
+    return m & ~lost;
+  }
+  __device__ __forceinline__ void apply(float scale, float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = reaches(j) ? v[j] * scale : 0.f;
+    if (lost != 0) {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (lost >> j & 1) v[j] = 0.f;
+    }
+  }
+};
+
+// the bits of one group of eight columns
+__device__ __forceinline__ unsigned kept8(const Drop& D, const DropKey& K, unsigned row, unsigned group) {
+  uint4 c[1] = {make_uint4(group, row, K.o0, K.o1)};
+  philox(c, K.k0, K.k1);
+  Bits8 b;
+  b.set(c[0], D, K, row, group);
+  return b.mask();
 }
 #endif
 
@@ -182,8 +266,8 @@ int check_vectors(const lmg_vectors* v, int width, const char* name);
 int check_drop(const lmg_dropout_spec* d);
 int check_index(const lmg_slots* s, int ntypes);
 Slots to_slots(const lmg_slots* s, int ntypes);
-Drop to_drop(const lmg_dropout_spec* d);  // threshold_hi and _lo 0: nothing is dropped
-inline bool drops(const Drop& D) { return D.threshold_hi != 0 || D.threshold_lo != 0; }
+Drop to_drop(const lmg_dropout_spec* d);  // upper and lower 0: nothing is dropped
+inline bool drops(const Drop& D) { return D.upper != 0 || D.lower != 0; }
 size_t embed_backward_bytes(unsigned rows, int ntypes, int width);
 // f(T, O) for the element types of source and result, which agree or are float32 and 16 bits
 template <class F>
