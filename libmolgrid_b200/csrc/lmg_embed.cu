@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(256, 6) k_rows_aligned(RowArgs A, const T* src
 constexpr int FLAT = 2048;
 
 template <class T, class O, bool LOOKUP, bool DROP>
-__global__ void __launch_bounds__(256) k_rows_flat(RowArgs A, const T* src, O* out) {
+__global__ void __launch_bounds__(256, 6) k_rows_flat(RowArgs A, const T* src, O* out) {
   __shared__ unsigned kept[DROP ? FLAT / 32 : 1];
   __shared__ int types[LOOKUP ? FLAT : 1];
   const unsigned n = A.rows * (unsigned)A.width, e0 = blockIdx.x * FLAT, end = min(e0 + FLAT, n);
@@ -153,6 +153,17 @@ __global__ void __launch_bounds__(256) k_rows_flat(RowArgs A, const T* src, O* o
     __syncthreads();
   }
   wait_for_stream();
+  constexpr int N = 16 / sizeof(O), TURNS = FLAT / 256 / N;
+  const T* from = src + (LOOKUP ? 0 : (long long)A.first * A.width);
+  O* to = out + (long long)A.first * A.width;
+  Raw<T, N> raw[LOOKUP ? 1 : TURNS];  // on their way while the bits are made
+  if (!LOOKUP) {
+#pragma unroll
+    for (int j = 0; j < TURNS; j++) {
+      const unsigned e = e0 + (j * 256 + threadIdx.x) * N;
+      if (e < end) raw[j].load(from + e, 0, (int)min(end - e, (unsigned)N));
+    }
+  }
   if (LOOKUP)
     for (unsigned r = row0 + threadIdx.x; r <= row1; r += 256) types[r - row0] = slot_type(A.S, A.first + r);
   if (DROP) {
@@ -171,11 +182,8 @@ __global__ void __launch_bounds__(256) k_rows_flat(RowArgs A, const T* src, O* o
     }
   }
   if (LOOKUP || DROP) __syncthreads();
-  constexpr int N = 16 / sizeof(O);
-  const T* from = src + (LOOKUP ? 0 : (long long)A.first * A.width);
-  O* to = out + (long long)A.first * A.width;
 #pragma unroll
-  for (int j = 0; j < FLAT / 256 / N; j++) {
+  for (int j = 0; j < TURNS; j++) {
     const unsigned e = e0 + (j * 256 + threadIdx.x) * N;
     if (e >= end) break;
     const bool whole = e + N <= end;
@@ -196,11 +204,9 @@ __global__ void __launch_bounds__(256) k_rows_flat(RowArgs A, const T* src, O* o
           if (++col == (unsigned)A.width) col = 0, row++;
         }
       }
-    } else if (whole) {
-      load_cols<T, N>(from + e, 0, N, v);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; i++) v[i] = e + i < end ? to_float(from[e + i]) : 0.f;
+      for (int i = 0; i < N; i++) v[i] = raw[LOOKUP ? 0 : j].get(i);
     }
     if (DROP) {
       const unsigned bits = kept[(e - e0) / 32] >> ((e - e0) & 31);

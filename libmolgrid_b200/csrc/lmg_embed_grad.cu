@@ -451,13 +451,6 @@ Plan plan_for(unsigned rows, int V, int width) {
   return p;
 }
 
-// more shared memory than a launch has without asking, once for each kernel and device
-template <class... P>
-cudaError_t allow_smem(void (*kernel)(P...), size_t bytes) {
-  if (bytes <= 48 << 10) return cudaSuccess;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
 template <class T, class O>
 cudaError_t by_tables(const Slots& S, const Plan& p, const lmg_vectors* diff, const lmg_vectors* grad, int width, float scale, const Drop& D,
                       char* ws, long* launches, cudaStream_t st) {

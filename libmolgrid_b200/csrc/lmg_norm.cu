@@ -4,48 +4,155 @@
 namespace lmg {
 namespace {
 
-constexpr int VALUES = 8;                       // of a row that a thread holds in registers
-constexpr int BLOCK = 256;                      // threads of a block whose rows each lie within a warp
-constexpr int ROW_THREADS_MOST = 1024;          // of a row: 8192 columns
-constexpr int WIDE = VALUES * ROW_THREADS_MOST;  // beyond it rows are read more than once (k_norm_wide, ...)
+constexpr int BLOCK = 256;      // threads of a block whose rows each lie within a warp
+constexpr int WIDE = 8192;      // columns; beyond it rows are read more than once (k_norm_wide, ...)
+constexpr int MIDDLE = 2048;    // columns up to which a thread holds eight values of a row, sixteen beyond
+// rows that are in use or on their way; both arrays of the widest rows fit an SM: 3 x 2 x 32 KB of float32, 4 x 2 x 16 KB of 16 bits
+template <class T> constexpr int STAGES = sizeof(T) == 4 ? 3 : 4;
 
-// A row's values over its `n` threads: VEC, 16 bytes a thread and turn, else an element a thread and turn, so that
-// neighbouring threads always read neighbouring bytes.
-template <class T, bool VEC>
+__device__ __forceinline__ void copy_async(unsigned to, const void* from, unsigned bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <class T> __device__ __forceinline__ Pair unpack(unsigned w);
+template <> __device__ __forceinline__ Pair unpack<__nv_bfloat16>(unsigned w) { return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <> __device__ __forceinline__ Pair unpack<__half>(unsigned w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pair(f.x, f.y);
+}
+template <class T> __device__ __forceinline__ unsigned packed(Pair p);
+template <> __device__ __forceinline__ unsigned packed<__nv_bfloat16>(Pair p) {
+  float a, b;
+  split(p, a, b);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+template <> __device__ __forceinline__ unsigned packed<__half>(Pair p) {
+  float a, b;
+  split(p, a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+
+// A thread's VALUES values of the rows it works on, brought through shared memory by asynchronous copies of 16 bytes, so that rows under
+// way take no registers.  VEC: rows begin on 16 bytes, a turn is 16 bytes a thread, and a thread copies what it
+// reads itself and waits for no one.  Otherwise a turn is an element a thread; the row's threads copy the 16-byte pieces that
+// the row lies in, from the one before its first value to its end, and wait for one another.  Neighbouring threads always
+// touch neighbouring bytes.
+template <class T, bool VEC, int VALUES>
 struct Share {
-  static constexpr int PER = VEC ? 16 / sizeof(T) : 1;
-  static __device__ __forceinline__ int col(int thread, int n, int i) { return (thread + n * (i / PER)) * PER + i % PER; }
-  static __device__ __forceinline__ void load(const T* row, int thread, int n, int width, float (&v)[VALUES]) {
+  static constexpr int PER = VEC ? 16 / sizeof(T) : 1, COPIES = VALUES * sizeof(T) / 16;
+  int thread, n, width;
+  bool full;                // all its columns are the row's
+  unsigned size[COPIES];    // VEC: bytes of its copies
+  unsigned here, step;      // its first copy's place in a stage, from one to the next
+
+  // bytes of a stage for a block of `block` threads, `n` a row
+  static __host__ __device__ __forceinline__ unsigned bytes(unsigned block, unsigned n) { return block * COPIES * 16 + (VEC ? 0 : block / n * 32); }
+  __device__ __forceinline__ int col(int i) const { return (thread + n * (i / PER)) * PER + i % PER; }
+  __device__ __forceinline__ bool valid(int i) const { return col(i) < width; }
+
+  __device__ __forceinline__ Share(int thread_, int n_, unsigned sub, int width_) : thread(thread_), n(n_), width(width_) {
+    full = col(VALUES - 1) < width;
+    here = VEC ? threadIdx.x * 16 : sub * (n * COPIES * 16 + 32);
+    step = (VEC ? blockDim.x : n) * 16;
 #pragma unroll
-    for (int k = 0; k < VALUES; k += PER) {
-      const int c = col(thread, n, k);
-      if (VEC && c + PER <= width) {
-        const uint4 a = *reinterpret_cast<const uint4*>(row + c);
-        const T* e = reinterpret_cast<const T*>(&a);
+    for (int k = 0; k < COPIES; k++) {
+      const int left = (width - col(k * PER)) * (int)sizeof(T);
+      size[k] = left < 0 ? 0 : left < 16 ? left : 16;
+    }
+  }
+  __device__ __forceinline__ void fetch(unsigned stage, const T* row) const {
+    if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) v[k + i] = to_float(e[i]);
-      } else {
+      for (int k = 0; k < COPIES; k++) copy_async(stage + here + k * step, size[k] ? row + (thread + n * k) * PER : row, size[k]);
+    } else {
+      const char* from = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
+      const int all = (int)(reinterpret_cast<uintptr_t>(row) & 15) + width * (int)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < PER; i++) v[k + i] = c + i < width ? to_float(row[c + i]) : 0.f;
+      for (int k = 0; k <= COPIES; k++) {
+        const int at = (thread + n * k) * 16, left = all - at;
+        if (left > 0) copy_async(stage + here + at, from + at, left < 16 ? left : 16);
       }
     }
   }
-  static __device__ __forceinline__ void store(T* row, int thread, int n, int width, const float (&v)[VALUES]) {
+  __device__ __forceinline__ void take(const char* stage, const T* row, Pair (&v)[VALUES / 2]) const {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int k = 0; k < VALUES; k += PER) {
-      const int c = col(thread, n, k);
-      if (VEC && c + PER <= width) {
-        uint4 a;
-        T* e = reinterpret_cast<T*>(&a);
+      for (int k = 0; k < COPIES; k++) {  // what lies behind the row's end has been filled with zeros
+        const uint4 a = *reinterpret_cast<const uint4*>(stage + here + k * step);
+        if constexpr (sizeof(T) == 4) {
+          v[2 * k] = pair(__uint_as_float(a.x), __uint_as_float(a.y));
+          v[2 * k + 1] = pair(__uint_as_float(a.z), __uint_as_float(a.w));
+        } else {
+          v[4 * k] = unpack<T>(a.x), v[4 * k + 1] = unpack<T>(a.y), v[4 * k + 2] = unpack<T>(a.z), v[4 * k + 3] = unpack<T>(a.w);
+        }
+      }
+    } else {
+      const T* e = reinterpret_cast<const T*>(stage + here + (reinterpret_cast<uintptr_t>(row) & 15)) + thread;
+      float f[VALUES];
+      if (full) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) e[i] = from_float<T>(v[k + i]);
-        *reinterpret_cast<uint4*>(row + c) = a;
+        for (int i = 0; i < VALUES; i++) f[i] = to_float(e[n * i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-          if (c + i < width) row[c + i] = from_float<T>(v[k + i]);
+        for (int i = 0; i < VALUES; i++) f[i] = valid(i) ? to_float(e[n * i]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < VALUES; i += 2) v[i / 2] = pair(f[i], f[i + 1]);
+    }
+  }
+  __device__ __forceinline__ void store(T* row, const Pair (&v)[VALUES / 2]) const {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int k = 0; k < COPIES; k++) {
+        T* to = row + (thread + n * k) * PER;
+        uint4 a;
+        if constexpr (sizeof(T) == 4) {
+          float f[4];
+          split(v[2 * k], f[0], f[1]);
+          split(v[2 * k + 1], f[2], f[3]);
+          a = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        } else {
+          a = make_uint4(packed<T>(v[4 * k]), packed<T>(v[4 * k + 1]), packed<T>(v[4 * k + 2]), packed<T>(v[4 * k + 3]));
+        }
+        if (size[k] == 16) {
+          *reinterpret_cast<uint4*>(to) = a;
+        } else {
+          const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+          for (int i = 0; i < PER; i++)
+            if (i * sizeof(T) < size[k]) to[i] = e[i];
+        }
+      }
+    } else {
+      T* to = row + thread;
+#pragma unroll
+      for (int i = 0; i < VALUES; i += 2) {
+        float f0, f1;
+        split(v[i / 2], f0, f1);
+        if (full || valid(i)) to[n * i] = from_float<T>(f0);
+        if (full || valid(i + 1)) to[n * (i + 1)] = from_float<T>(f1);
       }
     }
+  }
+  // values that are not the row's to zero
+  __device__ __forceinline__ void cut(Pair (&v)[VALUES / 2]) const {
+    if (full) return;
+#pragma unroll
+    for (int i = 0; i < VALUES; i += 2) {
+      float f0, f1;
+      split(v[i / 2], f0, f1);
+      v[i / 2] = pair(valid(i) ? f0 : 0.f, valid(i + 1) ? f1 : 0.f);
+    }
+  }
+  template <class P>
+  __device__ __forceinline__ void parameters(const P* p, float otherwise, Pair (&w)[VALUES / 2]) const {
+#pragma unroll
+    for (int i = 0; i < VALUES; i += 2)
+      w[i / 2] = pair(p != nullptr && valid(i) ? to_float(p[col(i)]) : otherwise, p != nullptr && valid(i + 1) ? to_float(p[col(i + 1)]) : otherwise);
   }
 };
 
@@ -55,13 +162,16 @@ template <bool SPAN, int SUMS>
 struct RowSum {
   float (*part)[SUMS][32];
   int n, turn = 0;
-  __device__ __forceinline__ void operator()(float (&v)[SUMS]) {
+  __device__ __forceinline__ void lanes(float (&v)[SUMS], int from) {
 #pragma unroll
     for (int o = 16; o; o >>= 1)
-      if (SPAN || o < n) {
+      if (o < from) {
 #pragma unroll
         for (int s = 0; s < SUMS; s++) v[s] += __shfl_xor_sync(0xffffffffu, v[s], o);
       }
+  }
+  __device__ __forceinline__ void operator()(float (&v)[SUMS]) {
+    lanes(v, SPAN ? 32 : n);
     if (SPAN) {
       const int lane = threadIdx.x & 31, warps = blockDim.x / 32;
       float (*p)[32] = part[turn];
@@ -71,12 +181,11 @@ struct RowSum {
         for (int s = 0; s < SUMS; s++) p[s][threadIdx.x / 32] = v[s];
       }
       __syncthreads();
+      // each group of as many lanes as there are warps, rounded up to a power of two, adds up all of them
+      const int at = lane & (n - 1);
 #pragma unroll
-      for (int s = 0; s < SUMS; s++) {
-        v[s] = lane < warps ? p[s][lane] : 0.f;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v[s] += __shfl_xor_sync(0xffffffffu, v[s], o);
-      }
+      for (int s = 0; s < SUMS; s++) v[s] = at < warps ? p[s][at] : 0.f;
+      lanes(v, n);
     }
   }
 };
@@ -84,154 +193,232 @@ struct RowSum {
 struct NormArgs {
   Slots S;
   int width, threads;  // threads of a row: a power of two up to 32, or the block
+  int group;           // lanes that a sum goes over at the end: `threads`, or the block's warps rounded up to a power of two
   unsigned tiles;      // of blockDim / threads rows
   float eps;
 };
 
+// The rows of a block one after the other: which of them hold anything, looked up a turn before their copies begin.
+struct Ahead {
+  unsigned rows, sub, filled = 0;  // bit k: the row k turns from now
+  int count = 0, place = 0;        // of the row whose copies come next
+  __device__ __forceinline__ void look(const NormArgs& A, unsigned tile) {
+    const unsigned row = tile * rows + sub;
+    place = 0;
+    count = tile < A.tiles && row < A.S.rows;
+    if (A.S.n_atoms != nullptr && count != 0) {
+      const unsigned b = A.S.by_n(row);
+      place = (int)(row - b * A.S.n);
+      count = A.S.n_atoms[b];
+    }
+  }
+  __device__ __forceinline__ bool there() const { return place < count; }
+};
+
 // Layer norm with the row in registers: mean, then the squares of what is left.  A block goes from row to row with its weights in
-// registers and the next row's loads under way.
-template <class T, class P, bool VEC, bool SPAN>
-__global__ void __launch_bounds__(SPAN ? 1024 : BLOCK) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
-                                                              long long out_ld, float* stats) {
-  typedef Share<T, VEC> Sh;
+// registers.  It is bound by what it issues where rows come from the L2: 16384 rows of 4096 bfloat16 took 91 us with eight values a thread,
+// one at a time and checked against the row's end (307 instructions a warp and row).
+template <class T, class P, bool VEC, bool SPAN, int VALUES>
+__global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
+                                                                     long long out_ld, float* stats) {
+  constexpr int H = VALUES / 2;
+  extern __shared__ __align__(16) char ring[];
   __shared__ float part[2][1][32];
   const int n = SPAN ? blockDim.x : A.threads, thread = SPAN ? threadIdx.x : threadIdx.x & (n - 1);
   const unsigned rows = SPAN ? 1 : BLOCK / n, sub = SPAN ? 0 : threadIdx.x / n;
-  RowSum<SPAN, 1> sum = {part, n};
+  const Share<T, VEC, VALUES> share(thread, n, sub, A.width);
+  const unsigned stage = share.bytes(blockDim.x, n), ring_at = (unsigned)__cvta_generic_to_shared(ring);
+  RowSum<SPAN, 1> sum = {part, A.group};
   wait_for_stream();
-  float w[VALUES], b[VALUES];
-#pragma unroll
-  for (int i = 0; i < VALUES; i++) {
-    const int c = Sh::col(thread, n, i);
-    w[i] = weight != nullptr && c < A.width ? to_float(weight[c]) : 1.f;
-    b[i] = bias != nullptr && c < A.width ? to_float(bias[c]) : 0.f;
-  }
-  const float inv = 1.f / (float)A.width;
-  float v[VALUES], next[VALUES];
-  auto fetch = [&](unsigned tile, float (&to)[VALUES]) {
-    const unsigned row = tile * rows + sub;
-    const bool there = tile < A.tiles && row < A.S.rows && slot_filled(A.S, row);
-    if (there) Sh::load(x + (long long)row * x_ld, thread, n, A.width, to);
-    return there;
+  Ahead ahead = {rows, sub};
+  unsigned coming = blockIdx.x;  // the tile whose copies come next
+  auto fetch = [&](int slot, int turn) {
+    const bool there = ahead.there();
+    if (there) share.fetch(ring_at + slot * stage, x + (long long)(coming * rows + sub) * x_ld);
+    copies_end_group();
+    ahead.filled |= (unsigned)there << turn;
+    coming += gridDim.x;
+    ahead.look(A, coming);
   };
-  bool there = fetch(blockIdx.x, v);
+  ahead.look(A, coming);
+#pragma unroll
+  for (int k = 0; k < STAGES<T> - 1; k++) fetch(k, k);
+  Pair w[H], b[H];
+  share.parameters(weight, 1.f, w);
+  share.parameters(bias, 0.f, b);
+  const float inv = 1.f / (float)A.width;
+  int slot = 0;
   for (unsigned tile = blockIdx.x; tile < A.tiles; tile += gridDim.x) {
-    const bool then = fetch(tile + gridDim.x, next);
+    if (!VEC && !SPAN) __syncwarp();  // the place that is filled next has been read
+    fetch(slot == 0 ? STAGES<T> - 1 : slot - 1, STAGES<T> - 1);
+    copies_but<STAGES<T> - 1>();
+    if (!VEC) {
+      if (SPAN) __syncthreads();
+      else __syncwarp();
+    }
+    const bool there = ahead.filled & 1;
+    ahead.filled >>= 1;
     const unsigned row = tile * rows + sub;
-    float s[1] = {0.f};
+    Pair v[H];
+    if (there) {
+      share.take(ring + slot * stage, x + (long long)row * x_ld, v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < VALUES; i++) {
-      if (!there) v[i] = 0.f;
-      s[0] += v[i];
+      for (int k = 0; k < H; k++) v[k] = pair(0.f);
     }
-    sum(s);
-    const float mean = s[0] * inv;
-    s[0] = 0.f;
+    slot = slot == STAGES<T> - 1 ? 0 : slot + 1;
+    float mean = 0.f, q = 0.f;
+    if (!SPAN || there) {
+      float s[1], t;
+      Pair a = v[0];
 #pragma unroll
-    for (int i = 0; i < VALUES; i++) {
-      v[i] = Sh::col(thread, n, i) < A.width ? v[i] - mean : 0.f;
-      s[0] += v[i] * v[i];
+      for (int k = 1; k < H; k++) a = add2(a, v[k]);
+      split(a, s[0], t);
+      s[0] += t;
+      sum(s);
+      mean = s[0] * inv;
+#pragma unroll
+      for (int k = 0; k < H; k++) v[k] = add2(v[k], pair(-mean));
+      share.cut(v);
+      a = mul2(v[0], v[0]);
+#pragma unroll
+      for (int k = 1; k < H; k++) a = fma2(v[k], v[k], a);
+      split(a, s[0], t);
+      s[0] += t;
+      sum(s);
+      q = rsqrtf(s[0] * inv + A.eps);
+      if (there) {
+#pragma unroll
+        for (int k = 0; k < H; k++) v[k] = fma2(mul2(v[k], pair(q)), w[k], b[k]);
+      }
     }
-    sum(s);
-    const float q = 1.f / sqrtf(s[0] * inv + A.eps);
     if (row < A.S.rows) {
-#pragma unroll
-      for (int i = 0; i < VALUES; i++) v[i] = there ? v[i] * q * w[i] + b[i] : 0.f;
-      Sh::store(out + (long long)row * out_ld, thread, n, A.width, v);
+      share.store(out + (long long)row * out_ld, v);
       if (stats != nullptr && thread == 0) reinterpret_cast<float2*>(stats)[row] = there ? make_float2(mean, q) : make_float2(0.f, 0.f);
     }
-    there = then;
-#pragma unroll
-    for (int i = 0; i < VALUES; i++) v[i] = next[i];
   }
+  copies_but<0>();
 }
 
 // dx = q (a - mean a - h mean(a h)) row by row, and with SUMS the sums over the block's rows of g h and g, which stay in the
 // registers of the threads that hold their columns: parts[block][2][width].
-template <class T, class P, bool VEC, bool SPAN, bool SUMS>
-__global__ void __launch_bounds__(SPAN ? 1024 : BLOCK) k_norm_backward(NormArgs A, const T* x, long long x_ld, const P* weight, const float* stats,
-                                                                       const T* diff, long long diff_ld, T* grad, long long grad_ld, float* parts) {
-  typedef Share<T, VEC> Sh;
+template <class T, class P, bool VEC, bool SPAN, int VALUES, bool SUMS>
+__global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm_backward(NormArgs A, const T* x, long long x_ld, const P* weight,
+                                                                              const float* stats, const T* diff, long long diff_ld, T* grad,
+                                                                              long long grad_ld, float* parts) {
+  constexpr int H = VALUES / 2;
+  extern __shared__ __align__(16) char ring[];
   __shared__ float part[2][2][32];
   const int n = SPAN ? blockDim.x : A.threads, thread = SPAN ? threadIdx.x : threadIdx.x & (n - 1);
   const unsigned rows = SPAN ? 1 : BLOCK / n, sub = SPAN ? 0 : threadIdx.x / n;
-  RowSum<SPAN, 2> sum = {part, n};
+  const Share<T, VEC, VALUES> share(thread, n, sub, A.width);
+  const unsigned stage = share.bytes(blockDim.x, n), ring_at = (unsigned)__cvta_generic_to_shared(ring);
+  RowSum<SPAN, 2> sum = {part, A.group};
   wait_for_stream();
-  float w[VALUES], dw[VALUES] = {}, db[VALUES] = {};
-#pragma unroll
-  for (int i = 0; i < VALUES; i++) {
-    const int c = Sh::col(thread, n, i);
-    w[i] = weight != nullptr && c < A.width ? to_float(weight[c]) : 1.f;
-  }
-  const float inv = 1.f / (float)A.width;
-  float v[VALUES], g[VALUES], next_v[VALUES], next_g[VALUES];
-  float2 st, next_st;
-  auto fetch = [&](unsigned tile, float (&to_v)[VALUES], float (&to_g)[VALUES], float2& to_st) {
-    const unsigned row = tile * rows + sub;
-    const bool there = tile < A.tiles && row < A.S.rows && slot_filled(A.S, row);
+  Ahead ahead = {rows, sub};
+  unsigned coming = blockIdx.x;
+  auto fetch = [&](int slot, int turn) {
+    const bool there = ahead.there();
     if (there) {
-      Sh::load(x + (long long)row * x_ld, thread, n, A.width, to_v);
-      Sh::load(diff + (long long)row * diff_ld, thread, n, A.width, to_g);
-      to_st = reinterpret_cast<const float2*>(stats)[row];
+      const long long row = coming * rows + sub;
+      share.fetch(ring_at + 2 * slot * stage, x + row * x_ld);
+      share.fetch(ring_at + (2 * slot + 1) * stage, diff + row * diff_ld);
     }
-    return there;
+    copies_end_group();
+    ahead.filled |= (unsigned)there << turn;
+    coming += gridDim.x;
+    ahead.look(A, coming);
   };
-  bool there = fetch(blockIdx.x, v, g, st);
+  ahead.look(A, coming);
+#pragma unroll
+  for (int k = 0; k < STAGES<T> - 1; k++) fetch(k, k);
+  Pair w[H], dw[H], db[H];
+  share.parameters(weight, 1.f, w);
+#pragma unroll
+  for (int k = 0; k < H; k++) dw[k] = db[k] = pair(0.f);
+  const float inv = 1.f / (float)A.width;
+  float2 st_next = make_float2(0.f, 0.f);
+  if (ahead.filled & 1) st_next = reinterpret_cast<const float2*>(stats)[blockIdx.x * rows + sub];
+  int slot = 0;
   for (unsigned tile = blockIdx.x; tile < A.tiles; tile += gridDim.x) {
-    const bool then = fetch(tile + gridDim.x, next_v, next_g, next_st);
+    if (!VEC && !SPAN) __syncwarp();
+    fetch(slot == 0 ? STAGES<T> - 1 : slot - 1, STAGES<T> - 1);
+    const float2 st = st_next;
+    if (ahead.filled & 2) st_next = reinterpret_cast<const float2*>(stats)[(tile + gridDim.x) * rows + sub];
+    copies_but<STAGES<T> - 1>();
+    if (!VEC) {
+      if (SPAN) __syncthreads();
+      else __syncwarp();
+    }
+    const bool there = ahead.filled & 1;
+    ahead.filled >>= 1;
     const unsigned row = tile * rows + sub;
-    float s[2] = {0.f, 0.f};
+    Pair v[H], g[H];
+    if (there) {
+      share.take(ring + 2 * slot * stage, x + (long long)row * x_ld, v);
+      share.take(ring + (2 * slot + 1) * stage, diff + (long long)row * diff_ld, g);
+    } else {
 #pragma unroll
-    for (int i = 0; i < VALUES; i++) {
-      if (!there) v[i] = g[i] = 0.f;
-      else v[i] = (v[i] - st.x) * st.y;
-      if (SUMS) {
-        dw[i] += g[i] * v[i];
-        db[i] += g[i];
+      for (int k = 0; k < H; k++) v[k] = g[k] = pair(0.f);
+    }
+    slot = slot == STAGES<T> - 1 ? 0 : slot + 1;
+    if (!SPAN || there) {
+      float s[2], t;
+      Pair a = pair(0.f), c = pair(0.f);
+#pragma unroll
+      for (int k = 0; k < H; k++) {
+        v[k] = mul2(add2(v[k], pair(there ? -st.x : 0.f)), pair(there ? st.y : 0.f));
+        if (SUMS) {
+          dw[k] = fma2(g[k], v[k], dw[k]);
+          db[k] = add2(db[k], g[k]);
+        }
+        g[k] = mul2(g[k], w[k]);
+        a = add2(a, g[k]);
+        c = fma2(g[k], v[k], c);
       }
-      g[i] *= w[i];
-      s[0] += g[i];
-      s[1] += g[i] * v[i];
-    }
-    sum(s);
-    const float s0 = s[0] * inv, s1 = s[1] * inv;
-    if (row < A.S.rows) {
+      split(a, s[0], t);
+      s[0] += t;
+      split(c, s[1], t);
+      s[1] += t;
+      sum(s);
+      if (there) {
+        const float s0 = -s[0] * inv, s1 = -s[1] * inv;
 #pragma unroll
-      for (int i = 0; i < VALUES; i++) v[i] = there ? st.y * (g[i] - s0 - v[i] * s1) : 0.f;
-      Sh::store(grad + (long long)row * grad_ld, thread, n, A.width, v);
+        for (int k = 0; k < H; k++) v[k] = mul2(fma2(v[k], pair(s1), add2(g[k], pair(s0))), pair(st.y));
+      }
     }
-    there = then;
-    st = next_st;
-#pragma unroll
-    for (int i = 0; i < VALUES; i++) {
-      v[i] = next_v[i];
-      g[i] = next_g[i];
-    }
+    if (row < A.S.rows) share.store(grad + (long long)row * grad_ld, v);
   }
+  copies_but<0>();
   if (!SUMS) return;
   float* mine = parts + (size_t)blockIdx.x * 2 * A.width;
   if (SPAN) {
 #pragma unroll
-    for (int i = 0; i < VALUES; i++) {
-      const int c = Sh::col(thread, n, i);
-      if (c < A.width) {
-        mine[c] = dw[i];
-        mine[A.width + c] = db[i];
-      }
+    for (int i = 0; i < VALUES; i += 2) {
+      float f0, f1;
+      split(dw[i / 2], f0, f1);
+      if (share.valid(i)) mine[share.col(i)] = f0;
+      if (share.valid(i + 1)) mine[share.col(i + 1)] = f1;
+      split(db[i / 2], f0, f1);
+      if (share.valid(i)) mine[A.width + share.col(i)] = f0;
+      if (share.valid(i + 1)) mine[A.width + share.col(i + 1)] = f1;
     }
   } else {
     // rows of a warp, then the warps
     __shared__ float all[2][BLOCK / 32][VALUES * 32];
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < VALUES; i++) {
+    for (int i = 0; i < VALUES; i += 2) {
+      float f[4];
+      split(dw[i / 2], f[0], f[1]);
+      split(db[i / 2], f[2], f[3]);
       for (int o = 16; o >= n; o >>= 1) {
-        dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-        db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+#pragma unroll
+        for (int k = 0; k < 4; k++) f[k] += __shfl_xor_sync(0xffffffffu, f[k], o);
       }
-      const int lane = threadIdx.x & 31;
       if (lane < n) {
-        all[0][threadIdx.x / 32][Sh::col(lane, n, i)] = dw[i];
-        all[1][threadIdx.x / 32][Sh::col(lane, n, i)] = db[i];
+#pragma unroll
+        for (int k = 0; k < 4; k++) all[k / 2][threadIdx.x / 32][share.col(i + k % 2)] = f[k];
       }
     }
     __syncthreads();
@@ -257,7 +444,7 @@ __global__ void __launch_bounds__(1024) k_norm_sums(const float* parts, int n, i
   float sum = 0.f;
   if (c < width) {
     const float* p = parts + (size_t)blockIdx.y * width + c;
-#pragma unroll 4
+#pragma unroll 8
     for (int k = slice; k < n; k += 32) sum += p[(size_t)k * 2 * width];
   }
   s[slice][threadIdx.x & 31] = sum;
@@ -276,7 +463,7 @@ template <class T, class P>
 __global__ void __launch_bounds__(WIDE_THREADS) k_norm_wide(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
                                                             long long out_ld, float* stats) {
   __shared__ float part[2][1][32];
-  RowSum<true, 1> sum = {part, WIDE_THREADS};
+  RowSum<true, 1> sum = {part, WIDE_THREADS / 32};
   wait_for_stream();
   const unsigned row = blockIdx.x;
   const T* in = x + (long long)row * x_ld;
@@ -311,7 +498,7 @@ template <class T, class P>
 __global__ void __launch_bounds__(WIDE_THREADS) k_norm_backward_wide(NormArgs A, const T* x, long long x_ld, const P* weight, const float* stats,
                                                                      const T* diff, long long diff_ld, T* grad, long long grad_ld) {
   __shared__ float part[2][2][32];
-  RowSum<true, 2> sum = {part, WIDE_THREADS};
+  RowSum<true, 2> sum = {part, WIDE_THREADS / 32};
   wait_for_stream();
   const unsigned row = blockIdx.x;
   const T* in = x + (long long)row * x_ld;
@@ -365,9 +552,9 @@ __global__ void __launch_bounds__(256) k_norm_weights_wide(NormArgs A, unsigned 
 // ---- the plan: a function of the sizes alone ------------------------------------------------------------------------------------
 struct NormPlan {
   bool wide;
-  int threads, block;      // of a row, of a block
-  unsigned tiles, blocks;  // blocks: of the backward pass, whose sums are apart
-  unsigned per;            // rows of a block of the wide sums
+  int values, threads, block, group;  // a thread's values of a row; threads of a row, of a block; see NormArgs
+  unsigned tiles, forward, blocks;    // blocks of the two passes; the sums of the backward pass go by its blocks
+  unsigned per;                       // rows of a block of the wide sums
   size_t bytes;
 };
 
@@ -378,17 +565,36 @@ NormPlan norm_plan(unsigned rows, int width) {
     p.blocks = rows / 64 < 1 ? 1 : rows / 64 > 64 ? 64 : rows / 64;
     p.per = (rows + p.blocks - 1) / p.blocks;
   } else {
+    p.values = width > MIDDLE ? 16 : 8;
     p.threads = 1;
-    while (p.threads < 32 && p.threads * VALUES < width) p.threads *= 2;
-    if (p.threads * VALUES < width) p.threads = (width + VALUES * 32 - 1) / (VALUES * 32) * 32;
+    while (p.threads < 32 && p.threads * p.values < width) p.threads *= 2;
+    if (p.threads * p.values < width) p.threads = (width + p.values * 32 - 1) / (p.values * 32) * 32;
     p.block = p.threads > 32 ? p.threads : BLOCK;
+    p.group = p.threads;
+    if (p.threads > 32)
+      for (p.group = 1; p.group < p.threads / 32;) p.group *= 2;
     const unsigned per = p.threads > 32 ? 1 : BLOCK / p.threads;
     p.tiles = (rows + per - 1) / per;
-    const unsigned resident = 148 * (unsigned)(1024 / p.block);
-    p.blocks = p.tiles < resident ? p.tiles : resident;
+    // blocks an SM holds: by the stages of float32, whatever the type, so that sums go by the sizes alone, and by registers
+    const size_t ring = (size_t)2 * STAGES<float> * p.block * p.values * 4;
+    auto fit = [&](size_t smem, int threads) {
+      const unsigned by_smem = (unsigned)((224 << 10) / (smem + 1024)), by_threads = threads > p.block ? threads / p.block : 1;
+      const unsigned all = 148 * (by_smem < by_threads ? by_smem : by_threads);
+      return p.tiles < all ? p.tiles : all;
+    };
+    p.blocks = fit(ring, p.values == 16 ? 512 : 1024);
+    p.forward = fit(ring / 2, p.values == 16 ? 1024 : 1536);
   }
   p.bytes = 256 + (size_t)p.blocks * 2 * width * 4;
   return p;
+}
+
+// dynamic shared memory of a pass over `arrays` arrays
+template <class T>
+size_t ring_bytes(const NormPlan& p, bool vec, int arrays) {
+  const unsigned stage = p.values == 16 ? (vec ? Share<T, true, 16>::bytes(p.block, p.threads) : Share<T, false, 16>::bytes(p.block, p.threads))
+                                        : (vec ? Share<T, true, 8>::bytes(p.block, p.threads) : Share<T, false, 8>::bytes(p.block, p.threads));
+  return (size_t)arrays * STAGES<T> * stage;
 }
 
 // F(T, P) for the element types of vectors and parameters, which agree or the latter are float32
@@ -397,6 +603,18 @@ cudaError_t by_types(int type, int weight_type, F f) {
   if (type == LMG_FLOAT32) return f(float(), float());
   if (type == LMG_BFLOAT16) return weight_type == LMG_FLOAT32 ? f(__nv_bfloat16(), float()) : f(__nv_bfloat16(), __nv_bfloat16());
   return weight_type == LMG_FLOAT32 ? f(__half(), float()) : f(__half(), __half());
+}
+
+template <class T, class P>
+auto by_plan(const NormPlan& p, bool vec, bool sums) {
+  if (p.values == 16)
+    return vec ? (sums ? k_norm_backward<T, P, true, true, 16, true> : k_norm_backward<T, P, true, true, 16, false>)
+               : (sums ? k_norm_backward<T, P, false, true, 16, true> : k_norm_backward<T, P, false, true, 16, false>);
+  if (p.threads > 32)
+    return vec ? (sums ? k_norm_backward<T, P, true, true, 8, true> : k_norm_backward<T, P, true, true, 8, false>)
+               : (sums ? k_norm_backward<T, P, false, true, 8, true> : k_norm_backward<T, P, false, true, 8, false>);
+  return vec ? (sums ? k_norm_backward<T, P, true, false, 8, true> : k_norm_backward<T, P, true, false, 8, false>)
+             : (sums ? k_norm_backward<T, P, false, false, 8, true> : k_norm_backward<T, P, false, false, 8, false>);
 }
 
 int check_weights(int type, int weight_type) {
@@ -430,18 +648,23 @@ int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const
   if ((rc = check_vectors(x, width, "input")) || (rc = check_vectors(out, width, "output"))) return rc;
   if (x->type != out->type) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "input and output differ in type");
   if ((rc = check_weights(x->type, weight_type)) || (rc = check_stats(stats))) return rc;
-  NormArgs A = {to_slots(rows, 0), width, 0, 0, eps};
+  NormArgs A = {to_slots(rows, 0), width, 0, 0, 0, eps};
   const NormPlan p = norm_plan(A.S.rows, width);
   A.threads = p.threads;
+  A.group = p.group;
   A.tiles = p.tiles;
   const bool vec = rows_aligned(x) && rows_aligned(out);
   const cudaError_t e = by_types(x->type, weight_type, [&](auto t, auto q) {
     typedef decltype(t) T;
     typedef decltype(q) P;
     auto kernel = k_norm_wide<T, P>;
-    if (!p.wide && p.threads > 32) kernel = vec ? k_norm<T, P, true, true> : k_norm<T, P, false, true>;
-    else if (!p.wide) kernel = vec ? k_norm<T, P, true, false> : k_norm<T, P, false, false>;
-    return launch_early(kernel, dim3(p.wide ? A.S.rows : p.blocks), p.wide ? WIDE_THREADS : p.block, 0, (cudaStream_t)stream, A,
+    if (!p.wide && p.values == 16) kernel = vec ? k_norm<T, P, true, true, 16> : k_norm<T, P, false, true, 16>;
+    else if (!p.wide && p.threads > 32) kernel = vec ? k_norm<T, P, true, true, 8> : k_norm<T, P, false, true, 8>;
+    else if (!p.wide) kernel = vec ? k_norm<T, P, true, false, 8> : k_norm<T, P, false, false, 8>;
+    const size_t ring = p.wide ? 0 : ring_bytes<T>(p, vec, 1);
+    const cudaError_t e = allow_smem(kernel, ring);
+    if (e != cudaSuccess) return e;
+    return launch_early(kernel, dim3(p.wide ? A.S.rows : p.forward), p.wide ? WIDE_THREADS : p.block, ring, (cudaStream_t)stream, A,
                         static_cast<const T*>(x->data), x->ld, static_cast<const P*>(weight), static_cast<const P*>(bias),
                         static_cast<T*>(out->data), out->ld, stats);
   });
@@ -470,9 +693,10 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
   } else if (weight_type < LMG_FLOAT32 || weight_type > LMG_FLOAT16) {
     return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "weights of unknown element type");
   }
-  NormArgs A = {to_slots(rows, 0), width, 0, 0, 0.f};
+  NormArgs A = {to_slots(rows, 0), width, 0, 0, 0, 0.f};
   const NormPlan p = norm_plan(A.S.rows, width);
   A.threads = p.threads;
+  A.group = p.group;
   A.tiles = p.tiles;
   if (workspace == nullptr || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return vectors_fail(LMG_ERR_WORKSPACE, "workspace too small for the gradients of a layer norm, or off 16 bytes");
@@ -501,17 +725,11 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
       e = launch_early(k_norm_backward_wide<T, P>, dim3(A.S.rows), WIDE_THREADS, 0, st, A, xp, x->ld, static_cast<const P*>(weight), stats, gp,
                        diff->ld, to, x_gradients->ld);
     } else {
-      auto kernel = k_norm_backward<T, P, false, false, false>;
-      const int which = (vec ? 4 : 0) + (p.threads > 32 ? 2 : 0) + (sums ? 1 : 0);
-      if (which == 1) kernel = k_norm_backward<T, P, false, false, true>;
-      if (which == 2) kernel = k_norm_backward<T, P, false, true, false>;
-      if (which == 3) kernel = k_norm_backward<T, P, false, true, true>;
-      if (which == 4) kernel = k_norm_backward<T, P, true, false, false>;
-      if (which == 5) kernel = k_norm_backward<T, P, true, false, true>;
-      if (which == 6) kernel = k_norm_backward<T, P, true, true, false>;
-      if (which == 7) kernel = k_norm_backward<T, P, true, true, true>;
-      e = launch_early(kernel, dim3(p.blocks), p.block, 0, st, A, xp, x->ld, static_cast<const P*>(weight), stats, gp, diff->ld, to, x_gradients->ld,
-                       parts);
+      auto kernel = by_plan<T, P>(p, vec, sums);
+      const size_t ring = ring_bytes<T>(p, vec, 2);
+      if ((e = allow_smem(kernel, ring)) != cudaSuccess) return e;
+      e = launch_early(kernel, dim3(p.blocks), p.block, ring, st, A, xp, x->ld, static_cast<const P*>(weight), stats, gp, diff->ld, to,
+                       x_gradients->ld, parts);
     }
     if (e != cudaSuccess) return e;
     launches++;

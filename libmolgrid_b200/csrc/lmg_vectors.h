@@ -281,6 +281,13 @@ cudaError_t by_vector_types(int in, int out, F f) {
   return f(__half(), __half());
 }
 inline size_t element_bytes(int type) { return type == LMG_FLOAT32 ? 4 : 2; }
+// more shared memory than a launch has without asking: 48 KB, its own variables among them (17 KB at most here)
+template <class... P>
+cudaError_t allow_smem(void (*kernel)(P...), size_t bytes) {
+  if (bytes <= 31 << 10) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
 // rows of which any eight columns that begin at a multiple of eight lie on 16 bytes
 inline bool rows_aligned(const lmg_vectors* v) {
   return reinterpret_cast<uintptr_t>(v->data) % 16 == 0 && v->ld * element_bytes(v->type) % 16 == 0;
