@@ -277,8 +277,9 @@ int lmg_sum_types(const float* type_index, const float* type_vector, int n, int 
  * none of this; a type vector is an input there (include/libmolgrid/coordinateset.h:30-39).
  *
  * Vectors are float32, bfloat16 or float16; every product and sum is float32 and a result is rounded
- * once.  A row has unit stride inside, rows lie `ld` elements apart (ld >= width); elements between
- * rows are neither read nor written.  Outputs may not overlap inputs, except where a comment allows it. */
+ * once.  Which kernels a call takes, and with them the last bits of its sums, goes by its sizes and types and by the alignment of its
+ * arrays; the same call has the same bits again.  A row has unit stride inside, rows lie `ld` elements apart (ld >= width); elements between
+ * rows are not written.  Outputs may not overlap inputs, except where a comment allows it. */
 enum { LMG_FLOAT32 = 0, LMG_BFLOAT16 = 1, LMG_FLOAT16 = 2 }; /* of vectors */
 enum { LMG_INDEX_FLOAT32 = 0, LMG_INDEX_INT32 = 1, LMG_INDEX_INT64 = 2 }; /* of type indices */
 
@@ -320,7 +321,7 @@ int lmg_embed_types(const lmg_slots* slots, int ntypes, int width, const lmg_vec
 /* Gradient of lmg_embed_types with respect to the table: table_gradients[type][width] = scale * the sum of
  * the gradients diff[slot][width] of the type's slots, after the same dropout; types without a slot get 0.
  * 16-bit gradients may go into a float32 table; otherwise the two types agree.  The slots of a type are
- * summed in an order fixed by the sizes of the call: the same call has the same bits again. */
+ * summed in a fixed order. */
 int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, const lmg_vectors* diff, float scale,
                              const lmg_dropout_spec* drop, const lmg_vectors* table_gradients, void* workspace,
                              size_t workspace_bytes, void* stream);
@@ -334,7 +335,7 @@ int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const
                    int weight_type, float eps, const lmg_vectors* out, float* stats, void* stream);
 
 /* Gradients of lmg_layer_norm from diff, that of its output: x_gradients, and weight_gradients[width] and
- * bias_gradients[width] (either may be NULL), summed over the rows in an order fixed by the sizes of the call.
+ * bias_gradients[width] (either may be NULL), summed over the rows in a fixed order.
  * x, diff and x_gradients have the same type; weight and the gradients of weight and bias have weight_type.  Empty rows get 0 and
  * add nothing.  x_gradients may be diff. */
 int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors* x, const void* weight,

@@ -6,12 +6,15 @@ namespace {
 
 constexpr int BLOCK = 256;      // threads of a block whose rows each lie within a warp
 constexpr int WIDE = 8192;      // columns; beyond it rows are read more than once (k_norm_wide, ...)
-constexpr int MIDDLE = 2048;    // columns up to which a thread holds eight values of a row, sixteen beyond
+constexpr int NARROW = 256;     // columns up to which a thread holds eight values of a row, sixteen beyond
 // rows that are in use or on their way; both arrays of the widest rows fit an SM: 3 x 2 x 32 KB of float32, 4 x 2 x 16 KB of 16 bits
 template <class T> constexpr int STAGES = sizeof(T) == 4 ? 3 : 4;
 
 __device__ __forceinline__ void copy_async(unsigned to, const void* from, unsigned bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async8(unsigned to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -36,105 +39,74 @@ template <> __device__ __forceinline__ unsigned packed<__half>(Pair p) {
   return *reinterpret_cast<const unsigned*>(&h);
 }
 
-// A thread's VALUES values of the rows it works on, brought through shared memory by asynchronous copies of 16 bytes, so that rows under
-// way take no registers.  VEC: rows begin on 16 bytes, a turn is 16 bytes a thread, and a thread copies what it
-// reads itself and waits for no one.  Otherwise a turn is an element a thread; the row's threads copy the 16-byte pieces that
-// the row lies in, from the one before its first value to its end, and wait for one another.  Neighbouring threads always
-// touch neighbouring bytes.
-template <class T, bool VEC, int VALUES>
+// A thread's VALUES values of the rows it works on: whole pieces of 16 bytes of memory, so that it copies, reads and writes 16
+// bytes at a time and waits for no one else's copies.  Rows that do not begin on 16 bytes have their first columns `shift` values
+// into the first piece; rows of one thread are as many apart as it takes for all to begin alike.  Copies are asynchronous, into a
+// ring in shared memory: rows under way take no registers.
+template <class T, int VALUES>
 struct Share {
-  static constexpr int PER = VEC ? 16 / sizeof(T) : 1, COPIES = VALUES * sizeof(T) / 16;
-  int thread, n, width;
-  bool full;                // all its columns are the row's
-  unsigned size[COPIES];    // VEC: bytes of its copies
-  unsigned here, step;      // its first copy's place in a stage, from one to the next
+  static constexpr int PER = 16 / sizeof(T), PIECES = VALUES / PER;
+  int thread, n, width, shift;
+  bool full;              // all its values are the row's
+  unsigned whole;         // a bit for each piece that is the row's
+  unsigned size[PIECES];  // bytes up to the row's end
+  unsigned off[PIECES];   // from its first piece, in values
 
-  // bytes of a stage for a block of `block` threads, `n` a row
-  static __host__ __device__ __forceinline__ unsigned bytes(unsigned block, unsigned n) { return block * COPIES * 16 + (VEC ? 0 : block / n * 32); }
-  __device__ __forceinline__ int col(int i) const { return (thread + n * (i / PER)) * PER + i % PER; }
-  __device__ __forceinline__ bool valid(int i) const { return col(i) < width; }
+  static __host__ __device__ __forceinline__ unsigned bytes(unsigned block) { return block * PIECES * 16; }  // of a stage
+  __device__ __forceinline__ int col(int i) const { return (thread + n * (i / PER)) * PER + i % PER - shift; }
+  __device__ __forceinline__ bool valid(int i) const { return (unsigned)col(i) < (unsigned)width; }
 
-  __device__ __forceinline__ Share(int thread_, int n_, unsigned sub, int width_) : thread(thread_), n(n_), width(width_) {
-    full = col(VALUES - 1) < width;
-    here = VEC ? threadIdx.x * 16 : sub * (n * COPIES * 16 + 32);
-    step = (VEC ? blockDim.x : n) * 16;
+  __device__ __forceinline__ Share(int thread_, int n_, int shift_, int width_) : thread(thread_), n(n_), width(width_), shift(shift_) {
+    full = valid(0) && valid(VALUES - 1);
+    whole = 0;
 #pragma unroll
-    for (int k = 0; k < COPIES; k++) {
+    for (int k = 0; k < PIECES; k++) {
       const int left = (width - col(k * PER)) * (int)sizeof(T);
       size[k] = left < 0 ? 0 : left < 16 ? left : 16;
+      off[k] = left > 0 ? n * PER * k : 0;
+      whole |= (unsigned)(valid(k * PER) && valid(k * PER + PER - 1)) << k;
     }
   }
-  __device__ __forceinline__ void fetch(unsigned stage, const T* row) const {
-    if constexpr (VEC) {
+  // where its first piece of a row begins
+  template <class Q>
+  __device__ __forceinline__ Q* first(Q* row) const { return row - shift + (col(0) < width ? thread * PER : 0); }
+  __device__ __forceinline__ void fetch(unsigned stage, const T* at) const {
 #pragma unroll
-      for (int k = 0; k < COPIES; k++) copy_async(stage + here + k * step, size[k] ? row + (thread + n * k) * PER : row, size[k]);
-    } else {
-      const char* from = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
-      const int all = (int)(reinterpret_cast<uintptr_t>(row) & 15) + width * (int)sizeof(T);
-#pragma unroll
-      for (int k = 0; k <= COPIES; k++) {
-        const int at = (thread + n * k) * 16, left = all - at;
-        if (left > 0) copy_async(stage + here + at, from + at, left < 16 ? left : 16);
-      }
-    }
+    for (int k = 0; k < PIECES; k++) copy_async(stage + (threadIdx.x + k * blockDim.x) * 16, at + off[k], size[k]);
   }
-  __device__ __forceinline__ void take(const char* stage, const T* row, Pair (&v)[VALUES / 2]) const {
-    if constexpr (VEC) {
+  __device__ __forceinline__ void take(const char* stage, Pair (&v)[VALUES / 2]) const {
 #pragma unroll
-      for (int k = 0; k < COPIES; k++) {  // what lies behind the row's end has been filled with zeros
-        const uint4 a = *reinterpret_cast<const uint4*>(stage + here + k * step);
-        if constexpr (sizeof(T) == 4) {
-          v[2 * k] = pair(__uint_as_float(a.x), __uint_as_float(a.y));
-          v[2 * k + 1] = pair(__uint_as_float(a.z), __uint_as_float(a.w));
-        } else {
-          v[4 * k] = unpack<T>(a.x), v[4 * k + 1] = unpack<T>(a.y), v[4 * k + 2] = unpack<T>(a.z), v[4 * k + 3] = unpack<T>(a.w);
-        }
-      }
-    } else {
-      const T* e = reinterpret_cast<const T*>(stage + here + (reinterpret_cast<uintptr_t>(row) & 15)) + thread;
-      float f[VALUES];
-      if (full) {
-#pragma unroll
-        for (int i = 0; i < VALUES; i++) f[i] = to_float(e[n * i]);
+    for (int k = 0; k < PIECES; k++) {  // what lies behind the row's end has been filled with zeros
+      const uint4 a = *reinterpret_cast<const uint4*>(stage + (threadIdx.x + k * blockDim.x) * 16);
+      if constexpr (sizeof(T) == 4) {
+        v[2 * k] = pair(__uint_as_float(a.x), __uint_as_float(a.y));
+        v[2 * k + 1] = pair(__uint_as_float(a.z), __uint_as_float(a.w));
       } else {
-#pragma unroll
-        for (int i = 0; i < VALUES; i++) f[i] = valid(i) ? to_float(e[n * i]) : 0.f;
+        v[4 * k] = unpack<T>(a.x), v[4 * k + 1] = unpack<T>(a.y), v[4 * k + 2] = unpack<T>(a.z), v[4 * k + 3] = unpack<T>(a.w);
       }
-#pragma unroll
-      for (int i = 0; i < VALUES; i += 2) v[i / 2] = pair(f[i], f[i + 1]);
     }
+    cut(v);
   }
-  __device__ __forceinline__ void store(T* row, const Pair (&v)[VALUES / 2]) const {
-    if constexpr (VEC) {
+  __device__ __forceinline__ void store(T* at, const Pair (&v)[VALUES / 2]) const {
 #pragma unroll
-      for (int k = 0; k < COPIES; k++) {
-        T* to = row + (thread + n * k) * PER;
-        uint4 a;
-        if constexpr (sizeof(T) == 4) {
-          float f[4];
-          split(v[2 * k], f[0], f[1]);
-          split(v[2 * k + 1], f[2], f[3]);
-          a = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-        } else {
-          a = make_uint4(packed<T>(v[4 * k]), packed<T>(v[4 * k + 1]), packed<T>(v[4 * k + 2]), packed<T>(v[4 * k + 3]));
-        }
-        if (size[k] == 16) {
-          *reinterpret_cast<uint4*>(to) = a;
-        } else {
-          const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-          for (int i = 0; i < PER; i++)
-            if (i * sizeof(T) < size[k]) to[i] = e[i];
-        }
+    for (int k = 0; k < PIECES; k++) {
+      T* to = at + off[k];
+      uint4 a;
+      if constexpr (sizeof(T) == 4) {
+        float f[4];
+        split(v[2 * k], f[0], f[1]);
+        split(v[2 * k + 1], f[2], f[3]);
+        a = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+      } else {
+        a = make_uint4(packed<T>(v[4 * k]), packed<T>(v[4 * k + 1]), packed<T>(v[4 * k + 2]), packed<T>(v[4 * k + 3]));
       }
-    } else {
-      T* to = row + thread;
+      if (whole >> k & 1) {
+        *reinterpret_cast<uint4*>(to) = a;
+      } else {
+        const T* e = reinterpret_cast<const T*>(&a);
 #pragma unroll
-      for (int i = 0; i < VALUES; i += 2) {
-        float f0, f1;
-        split(v[i / 2], f0, f1);
-        if (full || valid(i)) to[n * i] = from_float<T>(f0);
-        if (full || valid(i + 1)) to[n * (i + 1)] = from_float<T>(f1);
+        for (int i = 0; i < PER; i++)
+          if (valid(k * PER + i)) to[i] = e[i];
       }
     }
   }
@@ -156,24 +128,30 @@ struct Share {
   }
 };
 
-// Sums over the threads of a row, the same for all of them: `n` lanes next to each other, or (SPAN) the whole block.  A block's
-// sums take turns with two places in shared memory, so one barrier a sum is enough.
-template <bool SPAN, int SUMS>
+// Sums over the threads of a row, the same for all of them: `n` lanes next to each other, or (SPAN) a block of up to WARPS warps.  A
+// block's sums take turns with two places in shared memory, so one barrier a sum is enough.
+template <bool SPAN, int SUMS, int WARPS = 16>
 struct RowSum {
   float (*part)[SUMS][32];
   int n, turn = 0;
-  __device__ __forceinline__ void lanes(float (&v)[SUMS], int from) {
+  __device__ __forceinline__ RowSum(float (*part_)[SUMS][32], int n_) : part(part_), n(n_) {
+    if (SPAN) {  // the places of warps that the block does not have
+      for (int i = threadIdx.x; i < 2 * SUMS * 32; i += blockDim.x) part[i / (SUMS * 32)][i / 32 % SUMS][i % 32] = 0.f;
+      __syncthreads();
+    }
+  }
+  template <int FROM>
+  static __device__ __forceinline__ void lanes(float (&v)[SUMS]) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
-      if (o < from) {
+    for (int o = FROM / 2; o; o >>= 1) {
 #pragma unroll
-        for (int s = 0; s < SUMS; s++) v[s] += __shfl_xor_sync(0xffffffffu, v[s], o);
-      }
+      for (int s = 0; s < SUMS; s++) v[s] += __shfl_xor_sync(0xffffffffu, v[s], o);
+    }
   }
   __device__ __forceinline__ void operator()(float (&v)[SUMS]) {
-    lanes(v, SPAN ? 32 : n);
     if (SPAN) {
-      const int lane = threadIdx.x & 31, warps = blockDim.x / 32;
+      lanes<32>(v);
+      const int lane = threadIdx.x & 31;
       float (*p)[32] = part[turn];
       turn ^= 1;
       if (lane == 0) {
@@ -181,11 +159,14 @@ struct RowSum {
         for (int s = 0; s < SUMS; s++) p[s][threadIdx.x / 32] = v[s];
       }
       __syncthreads();
-      // each group of as many lanes as there are warps, rounded up to a power of two, adds up all of them
-      const int at = lane & (n - 1);
 #pragma unroll
-      for (int s = 0; s < SUMS; s++) v[s] = at < warps ? p[s][at] : 0.f;
-      lanes(v, n);
+      for (int s = 0; s < SUMS; s++) v[s] = p[s][lane & (WARPS - 1)];
+      lanes<WARPS>(v);
+    } else {
+      for (int o = n >> 1; o; o >>= 1) {
+#pragma unroll
+        for (int s = 0; s < SUMS; s++) v[s] += __shfl_xor_sync(0xffffffffu, v[s], o);
+      }
     }
   }
 };
@@ -193,17 +174,16 @@ struct RowSum {
 struct NormArgs {
   Slots S;
   int width, threads;  // threads of a row: a power of two up to 32, or the block
-  int group;           // lanes that a sum goes over at the end: `threads`, or the block's warps rounded up to a power of two
   unsigned tiles;      // of blockDim / threads rows
   float eps;
 };
 
 // The rows of a block one after the other: which of them hold anything, looked up a turn before their copies begin.
 struct Ahead {
-  unsigned rows, sub, filled = 0;  // bit k: the row k turns from now
-  int count = 0, place = 0;        // of the row whose copies come next
-  __device__ __forceinline__ void look(const NormArgs& A, unsigned tile) {
-    const unsigned row = tile * rows + sub;
+  unsigned tile, row, rows;  // whose copies come next
+  unsigned filled;           // bit k: the row k turns from now
+  int count, place;
+  __device__ __forceinline__ void look(const NormArgs& A) {
     place = 0;
     count = tile < A.tiles && row < A.S.rows;
     if (A.S.n_atoms != nullptr && count != 0) {
@@ -212,61 +192,72 @@ struct Ahead {
       count = A.S.n_atoms[b];
     }
   }
-  __device__ __forceinline__ bool there() const { return place < count; }
+  __device__ __forceinline__ Ahead(const NormArgs& A, unsigned rows_, unsigned sub)
+      : tile(blockIdx.x), row(blockIdx.x * rows_ + sub), rows(rows_ * gridDim.x), filled(0) {
+    look(A);
+  }
+  // whether the next row's copies are to begin
+  __device__ __forceinline__ bool next(const NormArgs& A, int turn) {
+    const bool there = place < count;
+    filled |= (unsigned)there << turn;
+    tile += gridDim.x;
+    row += rows;
+    look(A);
+    return there;
+  }
 };
 
+// how many values before it the 16 bytes begin that a row begins in
+template <class T>
+__device__ __forceinline__ int shift_of(const T* row) { return (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T); }
+
 // Layer norm with the row in registers: mean, then the squares of what is left.  A block goes from row to row with its weights in
-// registers.  It is bound by what it issues where rows come from the L2: 16384 rows of 4096 bfloat16 took 91 us with eight values a thread,
-// one at a time and checked against the row's end (307 instructions a warp and row).
-template <class T, class P, bool VEC, bool SPAN, int VALUES>
-__global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
-                                                                     long long out_ld, float* stats) {
-  constexpr int H = VALUES / 2;
+// registers.  16384 rows of 4096 bfloat16: 104 us with the next row in registers; 91 us with the ring, bound by what it issued with eight
+// values a thread, one at a time and each checked against the row's end; 67 us with sixteen in pairs.
+template <class T, class P, bool SPAN, int VALUES>
+__global__ void __launch_bounds__(SPAN ? 512 : BLOCK) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
+                                                             long long out_ld, float* stats) {
+  constexpr int H = VALUES / 2, S = STAGES<T>;
   extern __shared__ __align__(16) char ring[];
   __shared__ float part[2][1][32];
   const int n = SPAN ? blockDim.x : A.threads, thread = SPAN ? threadIdx.x : threadIdx.x & (n - 1);
   const unsigned rows = SPAN ? 1 : BLOCK / n, sub = SPAN ? 0 : threadIdx.x / n;
-  const Share<T, VEC, VALUES> share(thread, n, sub, A.width);
-  const unsigned stage = share.bytes(blockDim.x, n), ring_at = (unsigned)__cvta_generic_to_shared(ring);
-  RowSum<SPAN, 1> sum = {part, A.group};
+  unsigned row = blockIdx.x * rows + sub;
+  const Share<T, VALUES> share(thread, n, shift_of(x + (long long)row * x_ld), A.width);
+  const unsigned stage = share.bytes(blockDim.x), ring_at = (unsigned)__cvta_generic_to_shared(ring);
+  RowSum<SPAN, 1> sum(part, n);
   wait_for_stream();
-  Ahead ahead = {rows, sub};
-  unsigned coming = blockIdx.x;  // the tile whose copies come next
-  auto fetch = [&](int slot, int turn) {
-    const bool there = ahead.there();
-    if (there) share.fetch(ring_at + slot * stage, x + (long long)(coming * rows + sub) * x_ld);
-    copies_end_group();
-    ahead.filled |= (unsigned)there << turn;
-    coming += gridDim.x;
-    ahead.look(A, coming);
-  };
-  ahead.look(A, coming);
+  const T* from = share.first(x + (long long)row * x_ld);
+  T* to = share.first(out + (long long)row * out_ld);
+  const long long x_jump = x_ld * rows * gridDim.x, out_jump = out_ld * rows * gridDim.x;
+  Ahead ahead(A, rows, sub);
 #pragma unroll
-  for (int k = 0; k < STAGES<T> - 1; k++) fetch(k, k);
+  for (int k = 0; k < S - 1; k++) {
+    if (ahead.next(A, k)) share.fetch(ring_at + k * stage, from);
+    copies_end_group();
+    from += x_jump;
+  }
   Pair w[H], b[H];
   share.parameters(weight, 1.f, w);
   share.parameters(bias, 0.f, b);
   const float inv = 1.f / (float)A.width;
-  int slot = 0;
+  unsigned at = 0, fill = (S - 1) * stage;  // the stage in use, and the one before it, which is filled next
   for (unsigned tile = blockIdx.x; tile < A.tiles; tile += gridDim.x) {
-    if (!VEC && !SPAN) __syncwarp();  // the place that is filled next has been read
-    fetch(slot == 0 ? STAGES<T> - 1 : slot - 1, STAGES<T> - 1);
-    copies_but<STAGES<T> - 1>();
-    if (!VEC) {
-      if (SPAN) __syncthreads();
-      else __syncwarp();
-    }
+    if (ahead.next(A, S - 1)) share.fetch(ring_at + fill, from);
+    copies_end_group();
+    from += x_jump;
+    copies_but<S - 1>();
     const bool there = ahead.filled & 1;
     ahead.filled >>= 1;
-    const unsigned row = tile * rows + sub;
     Pair v[H];
     if (there) {
-      share.take(ring + slot * stage, x + (long long)row * x_ld, v);
+      share.take(ring + at, v);
     } else {
 #pragma unroll
       for (int k = 0; k < H; k++) v[k] = pair(0.f);
     }
-    slot = slot == STAGES<T> - 1 ? 0 : slot + 1;
+    fill = at;
+    at = at == (S - 1) * stage ? 0 : at + stage;
     float mean = 0.f, q = 0.f;
     if (!SPAN || there) {
       float s[1], t;
@@ -277,8 +268,9 @@ __global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm(NormArgs A,
       s[0] += t;
       sum(s);
       mean = s[0] * inv;
+      const Pair minus = pair(-mean);
 #pragma unroll
-      for (int k = 0; k < H; k++) v[k] = add2(v[k], pair(-mean));
+      for (int k = 0; k < H; k++) v[k] = add2(v[k], minus);
       share.cut(v);
       a = mul2(v[0], v[0]);
 #pragma unroll
@@ -288,86 +280,87 @@ __global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm(NormArgs A,
       sum(s);
       q = rsqrtf(s[0] * inv + A.eps);
       if (there) {
+        const Pair qq = pair(q);
 #pragma unroll
-        for (int k = 0; k < H; k++) v[k] = fma2(mul2(v[k], pair(q)), w[k], b[k]);
+        for (int k = 0; k < H; k++) v[k] = fma2(mul2(v[k], qq), w[k], b[k]);
       }
     }
-    if (row < A.S.rows) {
-      share.store(out + (long long)row * out_ld, v);
+    if (SPAN || row < A.S.rows) {
+      share.store(to, v);
       if (stats != nullptr && thread == 0) reinterpret_cast<float2*>(stats)[row] = there ? make_float2(mean, q) : make_float2(0.f, 0.f);
     }
+    row += rows * gridDim.x;
+    to += out_jump;
   }
   copies_but<0>();
 }
 
 // dx = q (a - mean a - h mean(a h)) row by row, and with SUMS the sums over the block's rows of g h and g, which stay in the
 // registers of the threads that hold their columns: parts[block][2][width].
-template <class T, class P, bool VEC, bool SPAN, int VALUES, bool SUMS>
-__global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm_backward(NormArgs A, const T* x, long long x_ld, const P* weight,
-                                                                              const float* stats, const T* diff, long long diff_ld, T* grad,
-                                                                              long long grad_ld, float* parts) {
-  constexpr int H = VALUES / 2;
+template <class T, class P, bool SPAN, int VALUES, bool SUMS>
+__global__ void __launch_bounds__(SPAN ? 512 : BLOCK) k_norm_backward(NormArgs A, const T* x, long long x_ld, const P* weight, const float* stats,
+                                                                      const T* diff, long long diff_ld, T* grad, long long grad_ld, float* parts) {
+  constexpr int H = VALUES / 2, S = STAGES<T>;
   extern __shared__ __align__(16) char ring[];
   __shared__ float part[2][2][32];
   const int n = SPAN ? blockDim.x : A.threads, thread = SPAN ? threadIdx.x : threadIdx.x & (n - 1);
   const unsigned rows = SPAN ? 1 : BLOCK / n, sub = SPAN ? 0 : threadIdx.x / n;
-  const Share<T, VEC, VALUES> share(thread, n, sub, A.width);
-  const unsigned stage = share.bytes(blockDim.x, n), ring_at = (unsigned)__cvta_generic_to_shared(ring);
-  RowSum<SPAN, 2> sum = {part, A.group};
+  unsigned row = blockIdx.x * rows + sub;
+  const Share<T, VALUES> share(thread, n, shift_of(x + (long long)row * x_ld), A.width);
+  // a stage holds both arrays and, for every thread, its row's stats: one row ahead in registers they were waited for at each turn's end
+  // (16384 rows of 4096 bfloat16: 107 us instead of 76)
+  const unsigned array = share.bytes(blockDim.x), stage = 2 * array + blockDim.x * 8, ring_at = (unsigned)__cvta_generic_to_shared(ring);
+  RowSum<SPAN, 2> sum(part, n);
   wait_for_stream();
-  Ahead ahead = {rows, sub};
-  unsigned coming = blockIdx.x;
-  auto fetch = [&](int slot, int turn) {
-    const bool there = ahead.there();
-    if (there) {
-      const long long row = coming * rows + sub;
-      share.fetch(ring_at + 2 * slot * stage, x + row * x_ld);
-      share.fetch(ring_at + (2 * slot + 1) * stage, diff + row * diff_ld);
+  const T *x_from = share.first(x + (long long)row * x_ld), *g_from = share.first(diff + (long long)row * diff_ld);
+  T* to = share.first(grad + (long long)row * grad_ld);
+  const unsigned jump = rows * gridDim.x;
+  const long long x_jump = x_ld * jump, g_jump = diff_ld * jump, to_jump = grad_ld * jump;
+  const float* st_from = stats + 2ll * row;
+  Ahead ahead(A, rows, sub);
+  auto fetch = [&](unsigned fill, int turn) {
+    if (ahead.next(A, turn)) {
+      share.fetch(ring_at + fill, x_from);
+      share.fetch(ring_at + fill + array, g_from);
+      copy_async8(ring_at + fill + 2 * array + threadIdx.x * 8, st_from);
     }
     copies_end_group();
-    ahead.filled |= (unsigned)there << turn;
-    coming += gridDim.x;
-    ahead.look(A, coming);
+    x_from += x_jump;
+    g_from += g_jump;
+    st_from += 2 * jump;
   };
-  ahead.look(A, coming);
 #pragma unroll
-  for (int k = 0; k < STAGES<T> - 1; k++) fetch(k, k);
+  for (int k = 0; k < S - 1; k++) fetch(k * stage, k);
   Pair w[H], dw[H], db[H];
   share.parameters(weight, 1.f, w);
 #pragma unroll
   for (int k = 0; k < H; k++) dw[k] = db[k] = pair(0.f);
   const float inv = 1.f / (float)A.width;
-  float2 st_next = make_float2(0.f, 0.f);
-  if (ahead.filled & 1) st_next = reinterpret_cast<const float2*>(stats)[blockIdx.x * rows + sub];
-  int slot = 0;
+  unsigned at = 0, fill = (S - 1) * stage;
   for (unsigned tile = blockIdx.x; tile < A.tiles; tile += gridDim.x) {
-    if (!VEC && !SPAN) __syncwarp();
-    fetch(slot == 0 ? STAGES<T> - 1 : slot - 1, STAGES<T> - 1);
-    const float2 st = st_next;
-    if (ahead.filled & 2) st_next = reinterpret_cast<const float2*>(stats)[(tile + gridDim.x) * rows + sub];
-    copies_but<STAGES<T> - 1>();
-    if (!VEC) {
-      if (SPAN) __syncthreads();
-      else __syncwarp();
-    }
+    fetch(fill, S - 1);
+    copies_but<S - 1>();
     const bool there = ahead.filled & 1;
     ahead.filled >>= 1;
-    const unsigned row = tile * rows + sub;
     Pair v[H], g[H];
+    float2 st = make_float2(0.f, 0.f);
     if (there) {
-      share.take(ring + 2 * slot * stage, x + (long long)row * x_ld, v);
-      share.take(ring + (2 * slot + 1) * stage, diff + (long long)row * diff_ld, g);
+      share.take(ring + at, v);
+      share.take(ring + at + array, g);
+      st = *reinterpret_cast<const float2*>(ring + at + 2 * array + threadIdx.x * 8);
     } else {
 #pragma unroll
       for (int k = 0; k < H; k++) v[k] = g[k] = pair(0.f);
     }
-    slot = slot == STAGES<T> - 1 ? 0 : slot + 1;
+    fill = at;
+    at = at == (S - 1) * stage ? 0 : at + stage;
     if (!SPAN || there) {
       float s[2], t;
       Pair a = pair(0.f), c = pair(0.f);
+      const Pair minus = pair(-st.x), q = pair(st.y);
 #pragma unroll
       for (int k = 0; k < H; k++) {
-        v[k] = mul2(add2(v[k], pair(there ? -st.x : 0.f)), pair(there ? st.y : 0.f));
+        v[k] = mul2(add2(v[k], minus), q);
         if (SUMS) {
           dw[k] = fma2(g[k], v[k], dw[k]);
           db[k] = add2(db[k], g[k]);
@@ -382,12 +375,14 @@ __global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm_backward(No
       s[1] += t;
       sum(s);
       if (there) {
-        const float s0 = -s[0] * inv, s1 = -s[1] * inv;
+        const Pair s0 = pair(-s[0] * inv), s1 = pair(-s[1] * inv);
 #pragma unroll
-        for (int k = 0; k < H; k++) v[k] = mul2(fma2(v[k], pair(s1), add2(g[k], pair(s0))), pair(st.y));
+        for (int k = 0; k < H; k++) v[k] = mul2(fma2(v[k], s1, add2(g[k], s0)), q);
       }
     }
-    if (row < A.S.rows) share.store(grad + (long long)row * grad_ld, v);
+    if (SPAN || row < A.S.rows) share.store(to, v);
+    row += jump;
+    to += to_jump;
   }
   copies_but<0>();
   if (!SUMS) return;
@@ -404,31 +399,25 @@ __global__ void __launch_bounds__(VALUES == 16 ? 512 : BLOCK) k_norm_backward(No
       if (share.valid(i + 1)) mine[A.width + share.col(i + 1)] = f1;
     }
   } else {
-    // rows of a warp, then the warps
-    __shared__ float all[2][BLOCK / 32][VALUES * 32];
-    const int lane = threadIdx.x & 31;
+    // a row's threads after the other's, in the ring: [rows][width], the two sums one after the other
+    float* all = reinterpret_cast<float*>(ring);
+    for (int which = 0; which < 2; which++) {
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < VALUES; i += 2) {
-      float f[4];
-      split(dw[i / 2], f[0], f[1]);
-      split(db[i / 2], f[2], f[3]);
-      for (int o = 16; o >= n; o >>= 1) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) f[k] += __shfl_xor_sync(0xffffffffu, f[k], o);
+      for (int i = 0; i < VALUES; i += 2) {
+        float f0, f1;
+        split(which ? db[i / 2] : dw[i / 2], f0, f1);
+        if (share.valid(i)) all[sub * A.width + share.col(i)] = f0;
+        if (share.valid(i + 1)) all[sub * A.width + share.col(i + 1)] = f1;
       }
-      if (lane < n) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) all[k / 2][threadIdx.x / 32][share.col(i + k % 2)] = f[k];
+      __syncthreads();
+      // 256 threads add up `width` columns of `rows` rows: groups of threads take rows in turn, then the groups are added up
+      for (int c = threadIdx.x; c < A.width; c += BLOCK) {
+        float t = 0.f;
+#pragma unroll 8
+        for (unsigned r = 0; r < rows; r++) t += all[r * A.width + c];
+        mine[which * A.width + c] = t;
       }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < 2 * VALUES * n; c += BLOCK) {
-      const int which = c >= VALUES * n, at = c - which * VALUES * n;
-      if (at >= A.width) continue;
-      float t = 0.f;
-#pragma unroll
-      for (int k = 0; k < BLOCK / 32; k++) t += all[which][k][at];
-      mine[which * A.width + at] = t;
     }
   }
 }
@@ -463,7 +452,7 @@ template <class T, class P>
 __global__ void __launch_bounds__(WIDE_THREADS) k_norm_wide(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
                                                             long long out_ld, float* stats) {
   __shared__ float part[2][1][32];
-  RowSum<true, 1> sum = {part, WIDE_THREADS / 32};
+  RowSum<true, 1, WIDE_THREADS / 32> sum(part, 0);
   wait_for_stream();
   const unsigned row = blockIdx.x;
   const T* in = x + (long long)row * x_ld;
@@ -498,7 +487,7 @@ template <class T, class P>
 __global__ void __launch_bounds__(WIDE_THREADS) k_norm_backward_wide(NormArgs A, const T* x, long long x_ld, const P* weight, const float* stats,
                                                                      const T* diff, long long diff_ld, T* grad, long long grad_ld) {
   __shared__ float part[2][2][32];
-  RowSum<true, 2> sum = {part, WIDE_THREADS / 32};
+  RowSum<true, 2, WIDE_THREADS / 32> sum(part, 0);
   wait_for_stream();
   const unsigned row = blockIdx.x;
   const T* in = x + (long long)row * x_ld;
@@ -550,36 +539,37 @@ __global__ void __launch_bounds__(256) k_norm_weights_wide(NormArgs A, unsigned 
 }
 
 // ---- the plan: a function of the sizes alone ------------------------------------------------------------------------------------
+// Which kernels: by the sizes, and by `slack`, the values that the rows' first pieces of 16 bytes may have more than the rows.
 struct NormPlan {
   bool wide;
-  int values, threads, block, group;  // a thread's values of a row; threads of a row, of a block; see NormArgs
-  unsigned tiles, forward, blocks;    // blocks of the two passes; the sums of the backward pass go by its blocks
-  unsigned per;                       // rows of a block of the wide sums
+  int values, threads, block;       // a thread's values of a row; threads of a row, of a block
+  unsigned tiles, forward, blocks;  // blocks of the two passes; the sums of the backward pass go by its blocks
+  unsigned per;                     // rows of a block of the wide sums
   size_t bytes;
 };
 
-NormPlan norm_plan(unsigned rows, int width) {
+NormPlan norm_plan(unsigned rows, int width, int slack) {
   NormPlan p = {};
-  p.wide = width > WIDE;
+  p.wide = width + slack > WIDE;
   if (p.wide) {
     p.blocks = rows / 64 < 1 ? 1 : rows / 64 > 64 ? 64 : rows / 64;
     p.per = (rows + p.blocks - 1) / p.blocks;
   } else {
-    p.values = width > MIDDLE ? 16 : 8;
+    const int most = width + slack;
+    p.values = most > NARROW ? 16 : 8;
     p.threads = 1;
-    while (p.threads < 32 && p.threads * p.values < width) p.threads *= 2;
-    if (p.threads * p.values < width) p.threads = (width + p.values * 32 - 1) / (p.values * 32) * 32;
+    while (p.threads < 32 && p.threads * p.values < most) p.threads *= 2;
+    if (p.threads * p.values < most) p.threads = (most + p.values * 32 - 1) / (p.values * 32) * 32;
     p.block = p.threads > 32 ? p.threads : BLOCK;
-    p.group = p.threads;
-    if (p.threads > 32)
-      for (p.group = 1; p.group < p.threads / 32;) p.group *= 2;
     const unsigned per = p.threads > 32 ? 1 : BLOCK / p.threads;
     p.tiles = (rows + per - 1) / per;
-    // blocks an SM holds: by the stages of float32, whatever the type, so that sums go by the sizes alone, and by registers
-    const size_t ring = (size_t)2 * STAGES<float> * p.block * p.values * 4;
+    // blocks an SM holds: by the stages of float32, whatever the type, so that sums go by the sizes alone, and by registers.  148 and its
+    // multiples by a block's rows, or by 2: as many rows apart as it takes for a thread's rows to begin alike in their 16 bytes
+    const size_t ring = (size_t)STAGES<float> * p.block * (2 * p.values * 4 + 8);
     auto fit = [&](size_t smem, int threads) {
       const unsigned by_smem = (unsigned)((224 << 10) / (smem + 1024)), by_threads = threads > p.block ? threads / p.block : 1;
-      const unsigned all = 148 * (by_smem < by_threads ? by_smem : by_threads);
+      unsigned all = 148 * (by_smem < by_threads ? by_smem : by_threads);
+      if (per == 1 && slack) all = all / 8 * 8;
       return p.tiles < all ? p.tiles : all;
     };
     p.blocks = fit(ring, p.values == 16 ? 512 : 1024);
@@ -589,12 +579,22 @@ NormPlan norm_plan(unsigned rows, int width) {
   return p;
 }
 
+// Rows that begin alike in their 16 bytes wherever one thread meets them: those of one array and, for one row, of all arrays.  false: they are
+// the wide kernels'.
+bool alike(const lmg_vectors* a, const lmg_vectors* b) {
+  const size_t size = element_bytes(a->type);
+  return (reinterpret_cast<uintptr_t>(a->data) - reinterpret_cast<uintptr_t>(b->data)) % 16 == 0 && (size_t)(a->ld - b->ld) * size % 16 == 0;
+}
+
+NormPlan plan_of(unsigned rows, int width, const lmg_vectors* x, bool all_alike) {
+  if (!all_alike) return norm_plan(rows, width, WIDE);
+  return norm_plan(rows, width, rows_aligned(x) ? 0 : 16 / (int)element_bytes(x->type) - 1);
+}
+
 // dynamic shared memory of a pass over `arrays` arrays
 template <class T>
-size_t ring_bytes(const NormPlan& p, bool vec, int arrays) {
-  const unsigned stage = p.values == 16 ? (vec ? Share<T, true, 16>::bytes(p.block, p.threads) : Share<T, false, 16>::bytes(p.block, p.threads))
-                                        : (vec ? Share<T, true, 8>::bytes(p.block, p.threads) : Share<T, false, 8>::bytes(p.block, p.threads));
-  return (size_t)arrays * STAGES<T> * stage;
+size_t ring_bytes(const NormPlan& p, int arrays) {
+  return (size_t)STAGES<T> * (arrays * (p.values == 16 ? Share<T, 16>::bytes(p.block) : Share<T, 8>::bytes(p.block)) + (arrays == 2 ? p.block * 8 : 0));
 }
 
 // F(T, P) for the element types of vectors and parameters, which agree or the latter are float32
@@ -603,18 +603,6 @@ cudaError_t by_types(int type, int weight_type, F f) {
   if (type == LMG_FLOAT32) return f(float(), float());
   if (type == LMG_BFLOAT16) return weight_type == LMG_FLOAT32 ? f(__nv_bfloat16(), float()) : f(__nv_bfloat16(), __nv_bfloat16());
   return weight_type == LMG_FLOAT32 ? f(__half(), float()) : f(__half(), __half());
-}
-
-template <class T, class P>
-auto by_plan(const NormPlan& p, bool vec, bool sums) {
-  if (p.values == 16)
-    return vec ? (sums ? k_norm_backward<T, P, true, true, 16, true> : k_norm_backward<T, P, true, true, 16, false>)
-               : (sums ? k_norm_backward<T, P, false, true, 16, true> : k_norm_backward<T, P, false, true, 16, false>);
-  if (p.threads > 32)
-    return vec ? (sums ? k_norm_backward<T, P, true, true, 8, true> : k_norm_backward<T, P, true, true, 8, false>)
-               : (sums ? k_norm_backward<T, P, false, true, 8, true> : k_norm_backward<T, P, false, true, 8, false>);
-  return vec ? (sums ? k_norm_backward<T, P, true, false, 8, true> : k_norm_backward<T, P, true, false, 8, false>)
-             : (sums ? k_norm_backward<T, P, false, false, 8, true> : k_norm_backward<T, P, false, false, 8, false>);
 }
 
 int check_weights(int type, int weight_type) {
@@ -635,7 +623,13 @@ extern "C" {
 
 size_t lmg_vectors_workspace_bytes(int op, int rows, int ntypes, int width) {
   if (rows < 0 || ntypes < 0 || width < 0) return 0;
-  return op == LMG_OP_EMBED_BACKWARD ? lmg::embed_backward_bytes((unsigned)rows, ntypes, width) : lmg::norm_plan((unsigned)rows, width).bytes;
+  if (op == LMG_OP_EMBED_BACKWARD) return lmg::embed_backward_bytes((unsigned)rows, ntypes, width);
+  size_t most = lmg::norm_plan((unsigned)rows, width, lmg::WIDE).bytes;  // that of any alignment
+  for (int slack : {0, 3, 7}) {
+    const size_t bytes = lmg::norm_plan((unsigned)rows, width, slack).bytes;
+    if (bytes > most) most = bytes;
+  }
+  return most;
 }
 
 int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const void* weight, const void* bias, int weight_type,
@@ -648,20 +642,17 @@ int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const
   if ((rc = check_vectors(x, width, "input")) || (rc = check_vectors(out, width, "output"))) return rc;
   if (x->type != out->type) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "input and output differ in type");
   if ((rc = check_weights(x->type, weight_type)) || (rc = check_stats(stats))) return rc;
-  NormArgs A = {to_slots(rows, 0), width, 0, 0, 0, eps};
-  const NormPlan p = norm_plan(A.S.rows, width);
+  NormArgs A = {to_slots(rows, 0), width, 0, 0, eps};
+  const NormPlan p = plan_of(A.S.rows, width, x, alike(x, out));
   A.threads = p.threads;
-  A.group = p.group;
   A.tiles = p.tiles;
-  const bool vec = rows_aligned(x) && rows_aligned(out);
   const cudaError_t e = by_types(x->type, weight_type, [&](auto t, auto q) {
     typedef decltype(t) T;
     typedef decltype(q) P;
     auto kernel = k_norm_wide<T, P>;
-    if (!p.wide && p.values == 16) kernel = vec ? k_norm<T, P, true, true, 16> : k_norm<T, P, false, true, 16>;
-    else if (!p.wide && p.threads > 32) kernel = vec ? k_norm<T, P, true, true, 8> : k_norm<T, P, false, true, 8>;
-    else if (!p.wide) kernel = vec ? k_norm<T, P, true, false, 8> : k_norm<T, P, false, false, 8>;
-    const size_t ring = p.wide ? 0 : ring_bytes<T>(p, vec, 1);
+    if (!p.wide && p.threads > 32) kernel = k_norm<T, P, true, 16>;
+    else if (!p.wide) kernel = p.values == 16 ? k_norm<T, P, false, 16> : k_norm<T, P, false, 8>;
+    const size_t ring = p.wide ? 0 : ring_bytes<T>(p, 1);
     const cudaError_t e = allow_smem(kernel, ring);
     if (e != cudaSuccess) return e;
     return launch_early(kernel, dim3(p.wide ? A.S.rows : p.forward), p.wide ? WIDE_THREADS : p.block, ring, (cudaStream_t)stream, A,
@@ -693,10 +684,9 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
   } else if (weight_type < LMG_FLOAT32 || weight_type > LMG_FLOAT16) {
     return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "weights of unknown element type");
   }
-  NormArgs A = {to_slots(rows, 0), width, 0, 0, 0, 0.f};
-  const NormPlan p = norm_plan(A.S.rows, width);
+  NormArgs A = {to_slots(rows, 0), width, 0, 0, 0.f};
+  const NormPlan p = none ? norm_plan(0, width, 0) : plan_of(A.S.rows, width, x, alike(x, diff) && alike(x, x_gradients));
   A.threads = p.threads;
-  A.group = p.group;
   A.tiles = p.tiles;
   if (workspace == nullptr || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return vectors_fail(LMG_ERR_WORKSPACE, "workspace too small for the gradients of a layer norm, or off 16 bytes");
@@ -707,7 +697,7 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
     if (e == cudaSuccess && bias_gradients) e = cudaMemsetAsync(bias_gradients, 0, width * element_bytes(weight_type), st);
     return e == cudaSuccess ? LMG_OK : vectors_cuda(e, "gradients of a layer norm");
   }
-  const bool vec = rows_aligned(x) && rows_aligned(diff) && rows_aligned(x_gradients), sums = weight_gradients || bias_gradients;
+  const bool sums = weight_gradients || bias_gradients;
   float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
   long launches = 0;
   const cudaError_t e = by_types(x->type, weight_type, [&](auto t, auto q) {
@@ -725,8 +715,10 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
       e = launch_early(k_norm_backward_wide<T, P>, dim3(A.S.rows), WIDE_THREADS, 0, st, A, xp, x->ld, static_cast<const P*>(weight), stats, gp,
                        diff->ld, to, x_gradients->ld);
     } else {
-      auto kernel = by_plan<T, P>(p, vec, sums);
-      const size_t ring = ring_bytes<T>(p, vec, 2);
+      auto kernel = sums ? k_norm_backward<T, P, true, 16, true> : k_norm_backward<T, P, true, 16, false>;
+      if (p.threads <= 32 && p.values == 16) kernel = sums ? k_norm_backward<T, P, false, 16, true> : k_norm_backward<T, P, false, 16, false>;
+      else if (p.threads <= 32) kernel = sums ? k_norm_backward<T, P, false, 8, true> : k_norm_backward<T, P, false, 8, false>;
+      const size_t ring = ring_bytes<T>(p, 2);
       if ((e = allow_smem(kernel, ring)) != cudaSuccess) return e;
       e = launch_early(kernel, dim3(p.blocks), p.block, ring, st, A, xp, x->ld, static_cast<const P*>(weight), stats, gp, diff->ld, to,
                        x_gradients->ld, parts);

@@ -217,9 +217,12 @@ def test_layer_norm(case, affine):
     on = N.on[..., 0]
     plain.assert_near(stats[on][:, :1], N.mean[on], N.dmean[on])
     assert bool(((stats[on][:, 1:].double() / N.q[on] - 1).abs() <= N.dq[on] + 2 * plain.U).all())
-    bare = torch.empty_like(x)
+    bare, _ = guarded(lead + (W,), vt, pad, offset)       # last bits go by the arrays' alignment: the same call again
     lmg.layer_norm(x, w, b, bare, None, 1e-5, na)
     assert torch.equal(bare, out)
+    dense = torch.empty(lead + (W,), dtype=vt, device="cuda")
+    lmg.layer_norm(x, w, b, dense, None, 1e-5, na)
+    plain.assert_near(dense, *N.forward())
 
     dx, check = guarded(lead + (W,), vt, pad, offset)
     dw, check_w = guarded((1, W), pt)
@@ -229,12 +232,15 @@ def test_layer_norm(case, affine):
     for got, v, t in zip((dx, dw[0], db[0]), want, tol):
         plain.assert_near(got, v, t)
     check(), check_w(), check_b()
-    again = [torch.full_like(v, 3.0) for v in (dx, dw[0], db[0])]
+    again = [guarded(lead + (W,), vt, pad, offset)[0].fill_(3.0)] + [torch.full_like(v, 3.0) for v in (dw[0], db[0])]
     lmg.layer_norm_backward(x, w, stats, diff, *again, na)
     assert all(torch.equal(p, q) for p, q in zip((dx, dw[0], db[0]), again))
+    dense = torch.empty(lead + (W,), dtype=vt, device="cuda")
+    lmg.layer_norm_backward(x, w, stats, diff, dense, None, None, na)
+    plain.assert_near(dense, want[0], tol[0])
     # one of the sums alone, none of them, and in place
     for mask in ((1, 0), (0, 1), (0, 0)):
-        got = torch.empty_like(dx)
+        got, _ = guarded(lead + (W,), vt, pad, offset)
         alone = [torch.empty(W, dtype=pt, device="cuda") if m else None for m in mask]
         lmg.layer_norm_backward(x, w, stats, diff, got, *alone, na)
         assert torch.equal(got, dx)
