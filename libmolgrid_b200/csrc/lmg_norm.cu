@@ -6,7 +6,8 @@ namespace {
 
 constexpr int BLOCK = 256;      // threads of a block whose rows each lie within a warp
 constexpr int WIDE = 8192;      // columns; beyond it rows are read more than once (k_norm_wide, ...)
-constexpr int NARROW = 256;     // columns up to which a thread holds eight values of a row, sixteen beyond
+constexpr int NARROW = 64;      // columns up to which a thread holds eight values of a row, sixteen beyond: 100000 rows of 64 float32 13.5
+                                // and 14.0 us (gradients of x), 50000 of 128 bfloat16 10.6 and 8.9
 // rows that are in use or on their way; both arrays of the widest rows fit an SM: 3 x 2 x 32 KB of float32, 4 x 2 x 16 KB of 16 bits
 template <class T> constexpr int STAGES = sizeof(T) == 4 ? 3 : 4;
 
@@ -215,7 +216,7 @@ __device__ __forceinline__ int shift_of(const T* row) { return (int)(reinterpret
 // registers.  16384 rows of 4096 bfloat16: 104 us with the next row in registers; 91 us with the ring, bound by what it issued with eight
 // values a thread, one at a time and each checked against the row's end; 67 us with sixteen in pairs.
 template <class T, class P, bool SPAN, int VALUES>
-__global__ void __launch_bounds__(SPAN ? 512 : BLOCK) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
+__global__ void __maxnreg__(VALUES == 16 ? 80 : 64) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
                                                              long long out_ld, float* stats) {
   constexpr int H = VALUES / 2, S = STAGES<T>;
   extern __shared__ __align__(16) char ring[];
@@ -298,8 +299,8 @@ __global__ void __launch_bounds__(SPAN ? 512 : BLOCK) k_norm(NormArgs A, const T
 // dx = q (a - mean a - h mean(a h)) row by row, and with SUMS the sums over the block's rows of g h and g, which stay in the
 // registers of the threads that hold their columns: parts[block][2][width].
 template <class T, class P, bool SPAN, int VALUES, bool SUMS>
-__global__ void __launch_bounds__(SPAN ? 512 : BLOCK) k_norm_backward(NormArgs A, const T* x, long long x_ld, const P* weight, const float* stats,
-                                                                      const T* diff, long long diff_ld, T* grad, long long grad_ld, float* parts) {
+__global__ void __maxnreg__(VALUES == 16 ? 128 : 80) k_norm_backward(NormArgs A, const T* x, long long x_ld, const P* weight, const float* stats,
+                                                                      const T* diff, long long diff_ld, T* grad, long long grad_ld, float* parts, P* dweight, P* dbias) {
   constexpr int H = VALUES / 2, S = STAGES<T>;
   extern __shared__ __align__(16) char ring[];
   __shared__ float part[2][2][32];
@@ -386,17 +387,26 @@ __global__ void __launch_bounds__(SPAN ? 512 : BLOCK) k_norm_backward(NormArgs A
   }
   copies_but<0>();
   if (!SUMS) return;
+  // the block's sums, or the call's where one block does all
   float* mine = parts + (size_t)blockIdx.x * 2 * A.width;
+  auto put = [&](int which, int c, float v) {
+    if (gridDim.x > 1) {
+      mine[which * A.width + c] = v;
+    } else {
+      P* to = which ? dbias : dweight;
+      if (to != nullptr) to[c] = from_float<P>(v);
+    }
+  };
   if (SPAN) {
 #pragma unroll
     for (int i = 0; i < VALUES; i += 2) {
       float f0, f1;
       split(dw[i / 2], f0, f1);
-      if (share.valid(i)) mine[share.col(i)] = f0;
-      if (share.valid(i + 1)) mine[share.col(i + 1)] = f1;
+      if (share.valid(i)) put(0, share.col(i), f0);
+      if (share.valid(i + 1)) put(0, share.col(i + 1), f1);
       split(db[i / 2], f0, f1);
-      if (share.valid(i)) mine[A.width + share.col(i)] = f0;
-      if (share.valid(i + 1)) mine[A.width + share.col(i + 1)] = f1;
+      if (share.valid(i)) put(1, share.col(i), f0);
+      if (share.valid(i + 1)) put(1, share.col(i + 1), f1);
     }
   } else {
     // a row's threads after the other's, in the ring: [rows][width], the two sums one after the other
@@ -411,12 +421,19 @@ __global__ void __launch_bounds__(SPAN ? 512 : BLOCK) k_norm_backward(NormArgs A
         if (share.valid(i + 1)) all[sub * A.width + share.col(i + 1)] = f1;
       }
       __syncthreads();
-      // 256 threads add up `width` columns of `rows` rows: groups of threads take rows in turn, then the groups are added up
-      for (int c = threadIdx.x; c < A.width; c += BLOCK) {
+      // columns by as many threads as there are, a power of two of them a column, which take rows in turn
+      int together = 1;
+      while (together < 32 && A.width * together * 2 <= BLOCK) together *= 2;
+      const int part_of = threadIdx.x & (together - 1);
+      for (int c0 = 0; c0 < A.width; c0 += BLOCK / together) {
+        const int c = c0 + threadIdx.x / together;
         float t = 0.f;
+        if (c < A.width) {
 #pragma unroll 8
-        for (unsigned r = 0; r < rows; r++) t += all[r * A.width + c];
-        mine[which * A.width + c] = t;
+          for (unsigned r = part_of; r < rows; r += together) t += all[r * A.width + c];
+        }
+        for (int o = together >> 1; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (c < A.width && part_of == 0) put(which, c, t);
       }
     }
   }
@@ -543,7 +560,7 @@ __global__ void __launch_bounds__(256) k_norm_weights_wide(NormArgs A, unsigned 
 struct NormPlan {
   bool wide;
   int values, threads, block;       // a thread's values of a row; threads of a row, of a block
-  unsigned tiles, forward, blocks;  // blocks of the two passes; the sums of the backward pass go by its blocks
+  unsigned tiles, forward, blocks;  // blocks of the two passes
   unsigned per;                     // rows of a block of the wide sums
   size_t bytes;
 };
@@ -572,8 +589,9 @@ NormPlan norm_plan(unsigned rows, int width, int slack) {
       if (per == 1 && slack) all = all / 8 * 8;
       return p.tiles < all ? p.tiles : all;
     };
-    p.blocks = fit(ring, p.values == 16 ? 512 : 1024);
-    p.forward = fit(ring / 2, p.values == 16 ? 1024 : 1536);
+    p.blocks = fit(ring, p.values == 16 ? 512 : 768);
+    p.forward = fit(ring / 2, p.values == 16 ? 768 : 1024);
+    if (p.tiles <= 4) p.blocks = 1;  // which needs no other launch for its sums (2.8 us)
   }
   p.bytes = 256 + (size_t)p.blocks * 2 * width * 4;
   return p;
@@ -721,11 +739,11 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
       const size_t ring = ring_bytes<T>(p, 2);
       if ((e = allow_smem(kernel, ring)) != cudaSuccess) return e;
       e = launch_early(kernel, dim3(p.blocks), p.block, ring, st, A, xp, x->ld, static_cast<const P*>(weight), stats, gp, diff->ld, to,
-                       x_gradients->ld, parts);
+                       x_gradients->ld, parts, static_cast<P*>(weight_gradients), static_cast<P*>(bias_gradients));
     }
     if (e != cudaSuccess) return e;
     launches++;
-    if (!sums) return e;
+    if (!sums || (!p.wide && p.blocks == 1)) return e;
     launches++;
     return launch_early(k_norm_sums<P>, dim3((width + 31) / 32, 2), 1024, 0, st, parts, (int)p.blocks, width, static_cast<P*>(weight_gradients),
                         static_cast<P*>(bias_gradients));
