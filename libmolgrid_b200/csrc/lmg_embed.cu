@@ -100,7 +100,21 @@ __global__ void __launch_bounds__(256, 6) k_rows_aligned(RowArgs A, const T* src
   wait_for_stream();
   const unsigned first = blockIdx.x * (A.down * UNITS);
   if (LOOKUP) {
-    for (unsigned i = threadIdx.x; i < A.down * UNITS; i += blockDim.x) types[i] = first + i < A.rows ? slot_type(A.S, A.first + first + i) : -1;
+    for (unsigned i0 = threadIdx.x; i0 < A.down * UNITS; i0 += blockDim.x * UNITS) {
+      unsigned r[UNITS];
+      bool in[UNITS];
+      int t[UNITS];
+#pragma unroll
+      for (int k = 0; k < UNITS; k++) {
+        const unsigned i = i0 + k * blockDim.x;
+        r[k] = A.first + first + i;
+        in[k] = i < A.down * UNITS && first + i < A.rows;
+      }
+      slot_types(A.S, r, in, t);
+#pragma unroll
+      for (int k = 0; k < UNITS; k++)
+        if (i0 + k * blockDim.x < A.down * UNITS) types[i0 + k * blockDim.x] = t[k];
+    }
     __syncthreads();
   }
   const unsigned sub = A.by_across(threadIdx.x), g = blockIdx.y * A.across + threadIdx.x - sub * A.across;

@@ -51,11 +51,18 @@ __global__ void __launch_bounds__(512) k_type_tables(Slots S, unsigned per, cons
     unsigned keep[8];
     if (DROP) {
       // eight slots of four groups of eight columns a turn: a lane draws for one of them and hands its bits round
+      const unsigned group = blockIdx.y * (TABLE_COLS / 8) + lane % 4;
+      uint4 c[4];
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const unsigned bits = kept8(D, K, r0 + j * 4 + lane / 4, blockIdx.y * (TABLE_COLS / 8) + lane % 4);
+      for (int j = 0; j < 4; j++) c[j] = make_uint4(group, r0 + j * 8 + lane / 4, K.o0, K.o1);
+      philox(c, K.k0, K.k1);
 #pragma unroll
-        for (int h = 0; h < 2; h++) keep[j + h] = __shfl_sync(0xffffffffu, bits, (h * 4 + q) * 4 + l / 2) >> (l & 1) * 4;
+      for (int j = 0; j < 4; j++) {
+        Bits8 b;
+        b.set(c[j], D, K, r0 + j * 8 + lane / 4, group);
+        const unsigned bits = b.mask();
+#pragma unroll
+        for (int h = 0; h < 2; h++) keep[2 * j + h] = __shfl_sync(0xffffffffu, bits, (h * 4 + q) * 4 + l / 2) >> (l & 1) * 4;
       }
     }
 #pragma unroll
@@ -112,8 +119,8 @@ constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_TILE_MOS
 
 // what a launch of the sort clears on the way: a share of the table's gradient, with what is idle beside the tiles
 struct Clear {
-  char* p;
-  size_t bytes;  // of the share; 16 bytes each, the first on a boundary
+  char* p;       // on a boundary of 16 bytes
+  size_t bytes;  // even
 };
 
 struct SortArgs {
@@ -135,6 +142,19 @@ __device__ __forceinline__ unsigned sort_key(const SortArgs& A, unsigned i) {
 __device__ void clear_share(const Clear& C, unsigned block, unsigned blocks) {
   uint4* p = reinterpret_cast<uint4*>(C.p);
   for (size_t i = (size_t)block * SORT_THREADS + threadIdx.x; i < C.bytes / 16; i += (size_t)blocks * SORT_THREADS) p[i] = make_uint4(0, 0, 0, 0);
+  if (block == 0 && threadIdx.x < C.bytes % 16 / 2) reinterpret_cast<unsigned short*>(C.p + C.bytes / 16 * 16)[threadIdx.x] = 0;
+}
+
+// The lanes whose digit of `bits` bits is this lane's, among those with a slot.  By ballots: __match_any_sync took two thirds of the
+// sort's time (25551 slots, 9 bits: 18 us of 30 for the whole gradient).
+__device__ __forceinline__ unsigned same_digit(unsigned digit, int bits, bool slot) {
+  unsigned same = __ballot_sync(0xffffffffu, slot);
+  for (int b = 0; b < bits; b++) {
+    const bool set = digit >> b & 1;
+    const unsigned with = __ballot_sync(0xffffffffu, set);
+    same &= set ? with : ~with;
+  }
+  return same;
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_count(SortArgs A) {
@@ -197,9 +217,9 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(SortArgs A) {
   // how many of each digit every warp has
   const unsigned per = A.tile / SORT_WARPS, begin = blockIdx.x * A.tile + warp * per, end = min(begin + per, A.S.rows);
   for (unsigned i0 = begin; i0 < end; i0 += 32) {
-    const unsigned i = i0 + lane, d = i < end ? sort_key(A, i) >> A.shift & mask : ~0u;
-    const unsigned peers = __match_any_sync(0xffffffffu, d);
-    if (d != ~0u && (peers & ((1u << lane) - 1)) == 0) mine[d] += (unsigned short)__popc(peers);
+    const unsigned i = i0 + lane, d = i < end ? sort_key(A, i) >> A.shift & mask : 0;
+    const unsigned peers = same_digit(d, A.bits, i < end);
+    if (i < end && (peers & ((1u << lane) - 1)) == 0) mine[d] += (unsigned short)__popc(peers);
     __syncwarp();
   }
   __syncthreads();
@@ -214,11 +234,11 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(SortArgs A) {
   }
   __syncthreads();
   for (unsigned i0 = begin; i0 < end; i0 += 32) {
-    const unsigned i = i0 + lane, key = i < end ? sort_key(A, i) : 0, d = i < end ? key >> A.shift & mask : ~0u;
-    const unsigned peers = __match_any_sync(0xffffffffu, d), lower = peers & ((1u << lane) - 1);
-    const unsigned at = d != ~0u ? base[d] + mine[d] + __popc(lower) : ~0u;
+    const unsigned i = i0 + lane, key = i < end ? sort_key(A, i) : 0, d = key >> A.shift & mask;
+    const unsigned peers = same_digit(d, A.bits, i < end), lower = peers & ((1u << lane) - 1);
+    const unsigned at = i < end ? base[d] + mine[d] + __popc(lower) : ~0u;
     __syncwarp();
-    if (d != ~0u && lower == 0) mine[d] += (unsigned short)__popc(peers);
+    if (i < end && lower == 0) mine[d] += (unsigned short)__popc(peers);
     __syncwarp();
     if (at < A.S.rows) {  // always, for types that nobody changes meanwhile
       A.key_out[at] = key;
@@ -226,6 +246,141 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(SortArgs A) {
     }
   }
 }
+
+// ---- the sort of up to 32768 slots, in one launch -----------------------------------------------------------------------------
+// Eight blocks of a cluster hold an eighth of the slots each, four a thread, and read one another's counts in shared memory; the
+// other clusters of the launch clear the table's gradient meanwhile.  (Two launches a pass: 16384 slots of 50021 types 35 us,
+// 25551 of 350 types 16 us.)
+constexpr unsigned CLUSTER = 8, CLUSTER_KEYS = 4;
+
+struct ClusterSortArgs {
+  Slots S;
+  unsigned each;            // slots of a block, a multiple of SORT_THREADS
+  int passes, bits;
+  unsigned *key[2], *row[2];
+  Clear clear;
+};
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// what another block of the cluster has at the same place in its shared memory
+__device__ __forceinline__ unsigned cluster_load(const unsigned* p, unsigned rank) {
+  unsigned v;
+  const unsigned at = (unsigned)__cvta_generic_to_shared(p);
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}" : "=r"(v) : "r"(at), "r"(rank) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A) {
+  extern __shared__ unsigned sort_shared[];
+  __shared__ unsigned warp_sum[SORT_WARPS];
+  wait_for_stream();
+  if (blockIdx.x >= CLUSTER) return clear_share(A.clear, blockIdx.x - CLUSTER, gridDim.x - CLUSTER);
+  const unsigned bins = 1u << A.bits, mask = bins - 1, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, block = blockIdx.x;
+  unsigned* count = sort_shared;                                            // [bins] of this block
+  unsigned* base = count + bins;                                            // [bins] first place of a digit's slots here
+  unsigned short* all = reinterpret_cast<unsigned short*>(base + bins);     // [warps][bins]
+  unsigned short* mine = all + warp * bins;
+  const unsigned per = A.each / SORT_WARPS, begin = block * A.each + warp * per, turns = begin < A.S.rows ? min(per, A.S.rows - begin) : 0;
+  const unsigned lower = (1u << lane) - 1;
+  for (int pass = 0; pass < A.passes; pass++) {
+    const int shift = pass * A.bits;
+    unsigned key[CLUSTER_KEYS], row[CLUSTER_KEYS];
+    bool slot[CLUSTER_KEYS];
+#pragma unroll
+    for (unsigned k = 0; k < CLUSTER_KEYS; k++) {
+      row[k] = begin + k * 32 + lane;
+      slot[k] = k * 32 + lane < turns;
+    }
+    if (pass == 0) {
+      int t[CLUSTER_KEYS];
+      slot_types(A.S, row, slot, t);
+#pragma unroll
+      for (unsigned k = 0; k < CLUSTER_KEYS; k++) key[k] = t[k] < 0 ? (unsigned)A.S.ntypes : (unsigned)t[k];  // empty slots come last
+    } else {  // past the L1, which may hold what lay there before
+#pragma unroll
+      for (unsigned k = 0; k < CLUSTER_KEYS; k++) {
+        key[k] = slot[k] ? __ldcg(A.key[(pass - 1) & 1] + row[k]) : 0;
+        row[k] = slot[k] ? __ldcg(A.row[(pass - 1) & 1] + row[k]) : 0;
+      }
+    }
+    for (unsigned b = lane; b < bins; b += 32) mine[b] = 0;
+    __syncwarp();
+    unsigned peers[CLUSTER_KEYS];
+#pragma unroll
+    for (unsigned k = 0; k < CLUSTER_KEYS; k++) {
+      if (k * 32 < turns) {
+        const unsigned d = key[k] >> shift & mask;
+        peers[k] = same_digit(d, A.bits, slot[k]);
+        if (slot[k] && (peers[k] & lower) == 0) mine[d] += (unsigned short)__popc(peers[k]);
+        __syncwarp();
+      }
+    }
+    __syncthreads();
+    for (unsigned b = tid; b < bins; b += SORT_THREADS) {
+      unsigned at = 0;
+#pragma unroll
+      for (unsigned w0 = 0; w0 < SORT_WARPS; w0 += 16) {
+        unsigned short n[16];
+#pragma unroll
+        for (unsigned w = 0; w < 16; w++) n[w] = all[(w0 + w) * bins + b];
+#pragma unroll
+        for (unsigned w = 0; w < 16; w++) {
+          all[(w0 + w) * bins + b] = (unsigned short)at;
+          at += n[w];
+        }
+      }
+      count[b] = at;
+    }
+    cluster_arrive();
+    cluster_wait();
+    // digits' totals to their first places; a thread has two digits at most
+    unsigned sum[2] = {0, 0}, off[2] = {0, 0};
+    const unsigned b0 = bins > SORT_THREADS ? 2 * tid : tid, nb = bins > SORT_THREADS ? 2 : b0 < bins ? 1 : 0;
+    for (unsigned k = 0; k < nb; k++) {
+#pragma unroll
+      for (unsigned c = 0; c < CLUSTER; c++) {
+        const unsigned n = cluster_load(count + b0 + k, c);
+        sum[k] += n;
+        off[k] += c < block ? n : 0;
+      }
+    }
+    const bool last = pass == A.passes - 1;
+    __syncthreads();
+    if (last) cluster_arrive();  // the others' counts have been read: they may leave once all have come here
+    unsigned run = sum[0] + sum[1];
+    for (unsigned o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 31) warp_sum[warp] = run;
+    __syncthreads();
+    unsigned before = lane < warp ? warp_sum[lane] : 0;
+    before = __reduce_add_sync(0xffffffffu, before);
+    const unsigned first = run - sum[0] - sum[1] + before;
+    if (nb > 0) base[b0] = first + off[0];
+    if (nb > 1) base[b0 + 1] = first + sum[0] + off[1];
+    __syncthreads();
+    unsigned *key_out = A.key[pass & 1], *row_out = A.row[pass & 1];
+#pragma unroll
+    for (unsigned k = 0; k < CLUSTER_KEYS; k++) {
+      if (k * 32 < turns) {
+        const unsigned d = key[k] >> shift & mask, at = slot[k] ? base[d] + mine[d] + __popc(peers[k] & lower) : ~0u;
+        __syncwarp();
+        if (slot[k] && (peers[k] & lower) == 0) mine[d] += (unsigned short)__popc(peers[k]);
+        __syncwarp();
+        if (at < A.S.rows) {  // always, for types that nobody changes meanwhile
+          key_out[at] = key[k];
+          row_out[at] = row[k];
+        }
+      }
+    }
+    if (!last) cluster_arrive();  // this pass is written, and its counts have been read
+    cluster_wait();
+  }
+}
+
+size_t cluster_smem(int bits) { return (8 + 2 * SORT_WARPS) * ((size_t)1 << bits); }
 
 size_t sort_smem(int bits) {
   const size_t bins = (size_t)1 << bits, slices = bins < SORT_THREADS ? SORT_THREADS / bins : 1;
@@ -350,11 +505,16 @@ __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* gr
   const unsigned at = blockIdx.x * PIECE_THREADS + threadIdx.x, block = at / A.lanes, slots = PIECE_THREADS / A.lanes * A.piece;
   const int col = (blockIdx.y * A.lanes + at % A.lanes) * 8;
   if (block + 1 >= A.blocks || col >= A.width) return;
-  const unsigned begin = block * slots, end = begin + slots, type = A.key[end - 1];
-  if (type >= A.ntypes || A.key[end] != type || (begin > 0 && A.key[begin - 1] == type)) return;
-  float sum[8];
+  // all that a type which ends in the next block needs is on its way before it is known whether there is one
+  const unsigned begin = block * slots, end = begin + slots, type = A.key[end - 1], goes = A.key[end], came = begin > 0 ? A.key[begin - 1] : ~0u;
+  const unsigned after = block + 2 < A.blocks ? A.key[end + slots] : ~0u;
+  float sum[8], more[8];
   load_cols<float, 8, false>(A.parts + ((size_t)block * 2 + 1) * A.width, col, A.width, sum);
-  unsigned p = block + 1;
+  load_cols<float, 8, false>(A.parts + ((size_t)block + 1) * 2 * A.width, col, A.width, more);
+  if (type >= A.ntypes || goes != type || came == type) return;
+#pragma unroll
+  for (int c = 0; c < 8; c++) sum[c] += more[c];
+  unsigned p = after == type ? block + 2 : A.blocks;
   while (p + 4 <= A.blocks && A.key[(p + 3) * slots] == type) {
     float v[4][8];
 #pragma unroll
@@ -366,10 +526,9 @@ __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* gr
     p += 4;
   }
   for (; p < A.blocks && A.key[p * slots] == type; p++) {
-    float v[8];
-    load_cols<float, 8, false>(A.parts + (size_t)p * 2 * A.width, col, A.width, v);
+    load_cols<float, 8, false>(A.parts + (size_t)p * 2 * A.width, col, A.width, more);
 #pragma unroll
-    for (int c = 0; c < 8; c++) sum[c] += v[c];
+    for (int c = 0; c < 8; c++) sum[c] += more[c];
   }
 #pragma unroll
   for (int c = 0; c < 8; c++) sum[c] *= A.scale;
@@ -384,7 +543,7 @@ struct Plan {
   int warps;
   size_t table_smem;
   // sorted
-  unsigned tiles, tile;
+  unsigned tiles, tile;  // tiles 0: one cluster sorts, `tile` slots a block
   int passes, bits;
   unsigned piece, piece_blocks;
   int lanes;
@@ -418,21 +577,26 @@ Plan plan_for(unsigned rows, int V, int width) {
       return p;
     }
   }
-  p.tile = SORT_THREADS;
-  while ((rows + p.tile - 1) / p.tile > 148 && p.tile < SORT_TILE_MOST) p.tile += SORT_THREADS;
-  p.tiles = (rows + p.tile - 1) / p.tile;
   int key_bits = 1, most = 1;
   while (key_bits < 31 && (unsigned)V >> key_bits) key_bits++;
-  // a block reads all tiles' counts: half a megabyte at most
-  while (most < SORT_BITS_MOST && ((size_t)p.tiles << (most + 1)) <= 1 << 17) most++;
+  if (rows <= CLUSTER * CLUSTER_KEYS * SORT_THREADS) {
+    p.tile = (rows + CLUSTER * SORT_THREADS - 1) / (CLUSTER * SORT_THREADS) * SORT_THREADS;
+    most = SORT_BITS_MOST;
+  } else {
+    p.tile = SORT_THREADS;
+    while ((rows + p.tile - 1) / p.tile > 148 && p.tile < SORT_TILE_MOST) p.tile += SORT_THREADS;
+    p.tiles = (rows + p.tile - 1) / p.tile;
+    // a block reads all tiles' counts: half a megabyte at most
+    while (most < SORT_BITS_MOST && ((size_t)p.tiles << (most + 1)) <= 1 << 17) most++;
+  }
   p.passes = (key_bits + most - 1) / most;
   p.bits = (key_bits + p.passes - 1) / p.passes;
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes * 8 < width) p.lanes *= 2;
   const unsigned cols = (width + p.lanes * 8 - 1) / (p.lanes * 8);
-  // pieces for 64 warps an SM, of 8 to 32 slots
-  const size_t want = (size_t)rows * cols * p.lanes / (148 * 64 * 32);
-  p.piece = 8;
+  // pieces for 16 warps an SM, of 4 to 32 slots: for 64, 16384 slots of 1024 bfloat16 take 46 us instead of 42
+  const size_t want = (size_t)rows * cols * p.lanes / (148 * 16 * 32);
+  p.piece = 4;
   while (p.piece < 32 && p.piece < want && p.piece * 2 * (PIECE_THREADS / p.lanes) <= PIECE_SLOTS) p.piece *= 2;
   const unsigned slots = p.piece * (PIECE_THREADS / p.lanes);
   p.piece_blocks = (rows + slots - 1) / slots;
@@ -480,40 +644,54 @@ cudaError_t by_sort(const Slots& S, const Plan& p, const lmg_vectors* diff, cons
   cudaError_t e = cudaSuccess;
   const bool dense = grad->ld == width && reinterpret_cast<uintptr_t>(g) % 16 == 0;
   if (!dense) e = cudaMemset2DAsync(g, grad->ld * size, 0, width * size, S.ntypes, st);
-  else if (total % 16) e = cudaMemsetAsync(g + total / 16 * 16, 0, total % 16, st);
   if (e != cudaSuccess) return e;
-  const int parts = 2 * p.passes;
-  const size_t share = dense ? (total / 16 + parts - 1) / parts * 16 : 0;
-  SortArgs A = {};
-  A.S = S;
-  A.tiles = p.tiles;
-  A.tile = p.tile;
-  A.bits = p.bits;
-  A.counts = reinterpret_cast<unsigned*>(ws + p.counts);
-  const size_t smem = sort_smem(p.bits);
-  if ((e = allow_smem(k_sort_move, smem)) != cudaSuccess) return e;
-  auto clear = [&](int k) {
-    const size_t from = share * k < total / 16 * 16 ? share * k : total / 16 * 16;
-    A.clear.p = g + from;
-    A.clear.bytes = total / 16 * 16 - from < share ? total / 16 * 16 - from : share;
-    const size_t blocks = (A.clear.bytes / 16 + SORT_THREADS * 4 - 1) / (SORT_THREADS * 4);
-    return p.tiles + (unsigned)(blocks < 296 ? blocks : 296);
+  const int parts = p.tiles ? 2 * p.passes : 1;
+  const size_t clears = dense ? total : 0, share = (clears / 16 + parts) / parts * 16;
+  auto clear = [&](int k, Clear& c) {
+    const size_t from = share * k < clears ? share * k : clears;
+    c.p = g + from;
+    c.bytes = clears - from < share ? clears - from : share;
+    const size_t blocks = (c.bytes / 16 + SORT_THREADS * 4) / (SORT_THREADS * 4);
+    return c.bytes == 0 ? 0u : (unsigned)(blocks < 296 ? blocks : 296);
   };
-  for (int k = 0; k < p.passes; k++) {
-    A.shift = k * p.bits;
-    A.key_in = k ? reinterpret_cast<unsigned*>(ws + p.key[(k - 1) & 1]) : nullptr;
-    A.row_in = k ? reinterpret_cast<unsigned*>(ws + p.row[(k - 1) & 1]) : nullptr;
-    A.key_out = reinterpret_cast<unsigned*>(ws + p.key[k & 1]);
-    A.row_out = reinterpret_cast<unsigned*>(ws + p.row[k & 1]);
-    unsigned blocks = clear(2 * k);
-    if ((e = launch_early(k_sort_count, dim3(blocks), SORT_THREADS, 0, st, A)) != cudaSuccess) return e;
-    blocks = clear(2 * k + 1);
-    if ((e = launch_early(k_sort_move, dim3(blocks), SORT_THREADS, smem, st, A)) != cudaSuccess) return e;
-    *launches += 2;
+  unsigned *key[2], *row[2];
+  for (int k = 0; k < 2; k++) {
+    key[k] = reinterpret_cast<unsigned*>(ws + p.key[k]);
+    row[k] = reinterpret_cast<unsigned*>(ws + p.row[k]);
+  }
+  if (p.tiles == 0) {
+    ClusterSortArgs A = {S, p.tile, p.passes, p.bits, {key[0], key[1]}, {row[0], row[1]}, {}};
+    const unsigned blocks = clear(0, A.clear);
+    const size_t smem = cluster_smem(p.bits);
+    if ((e = allow_smem(k_sort_cluster, smem)) != cudaSuccess) return e;
+    e = launch_clusters(k_sort_cluster, CLUSTER + (blocks + CLUSTER - 1) / CLUSTER * CLUSTER, CLUSTER, SORT_THREADS, smem, st, A);
+    if (e != cudaSuccess) return e;
+    ++*launches;
+  } else {
+    SortArgs A = {};
+    A.S = S;
+    A.tiles = p.tiles;
+    A.tile = p.tile;
+    A.bits = p.bits;
+    A.counts = reinterpret_cast<unsigned*>(ws + p.counts);
+    const size_t smem = sort_smem(p.bits);
+    if ((e = allow_smem(k_sort_move, smem)) != cudaSuccess) return e;
+    for (int k = 0; k < p.passes; k++) {
+      A.shift = k * p.bits;
+      A.key_in = k ? key[(k - 1) & 1] : nullptr;
+      A.row_in = k ? row[(k - 1) & 1] : nullptr;
+      A.key_out = key[k & 1];
+      A.row_out = row[k & 1];
+      unsigned blocks = p.tiles + clear(2 * k, A.clear);
+      if ((e = launch_early(k_sort_count, dim3(blocks), SORT_THREADS, 0, st, A)) != cudaSuccess) return e;
+      blocks = p.tiles + clear(2 * k + 1, A.clear);
+      if ((e = launch_early(k_sort_move, dim3(blocks), SORT_THREADS, smem, st, A)) != cudaSuccess) return e;
+      *launches += 2;
+    }
   }
   PieceArgs P = {};
-  P.key = A.key_out;
-  P.row = A.row_out;
+  P.key = key[(p.passes - 1) & 1];
+  P.row = row[(p.passes - 1) & 1];
   P.n = S.rows;
   P.ntypes = (unsigned)S.ntypes;
   P.piece = p.piece;

@@ -53,28 +53,55 @@ __device__ __forceinline__ bool slot_filled(const Slots& S, unsigned row) {
   return (int)(row - b * S.n) < S.n_atoms[b];
 }
 
-// type of a slot, -1 where it is empty; its count and its index are on their way together
-__device__ __forceinline__ int slot_type(const Slots& S, unsigned row) {
-  bool filled = true, high;
-  int t;
-  if (S.n_atoms != nullptr) {
-    const unsigned b = S.by_n(row);
-    filled = (int)(row - b * S.n) < S.n_atoms[b];
-  }
+// types of N slots, -1 where one is empty (or `in` is false); all their counts and indices are on their way together
+template <int N>
+__device__ __forceinline__ void slot_types(const Slots& S, const unsigned (&row)[N], const bool (&in)[N], int (&t)[N]) {
   if (S.index_type == LMG_INDEX_FLOAT32) {
-    const float f = roundf(static_cast<const float*>(S.index)[row]);
-    t = f >= 0.f ? f < 2147483648.f ? (int)f : 0x7fffffff : -1;
-    high = t >= S.ntypes;
+    float f[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) f[k] = in[k] ? static_cast<const float*>(S.index)[row[k]] : -1.f;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      f[k] = roundf(f[k]);
+      t[k] = f[k] >= 0.f ? f[k] < 2147483648.f ? (int)f[k] : 0x7fffffff : -1;
+    }
   } else if (S.index_type == LMG_INDEX_INT32) {
-    t = static_cast<const int*>(S.index)[row];
-    high = t >= S.ntypes;
+#pragma unroll
+    for (int k = 0; k < N; k++) t[k] = in[k] ? static_cast<const int*>(S.index)[row[k]] : -1;
   } else {
-    const long long l = static_cast<const long long*>(S.index)[row];
-    high = l >= S.ntypes;
-    t = l < 0 ? -1 : (int)l;
+    long long l[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) l[k] = in[k] ? static_cast<const long long*>(S.index)[row[k]] : -1;
+#pragma unroll
+    for (int k = 0; k < N; k++) t[k] = l[k] < 0 ? -1 : l[k] < 0x7fffffff ? (int)l[k] : 0x7fffffff;
   }
-  if (filled && high && S.status != nullptr) *S.status = 1;
-  return filled && !high && t >= 0 ? t : -1;
+  if (S.n_atoms != nullptr) {
+    int place[N], count[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const unsigned b = S.by_n(in[k] ? row[k] : 0);
+      place[k] = (int)((in[k] ? row[k] : 0) - b * S.n);
+      count[k] = S.n_atoms[b];
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++)
+      if (place[k] >= count[k]) t[k] = -1;
+  }
+  bool high = false;
+#pragma unroll
+  for (int k = 0; k < N; k++)
+    if (t[k] >= S.ntypes) {
+      high = true;
+      t[k] = -1;
+    }
+  if (high && S.status != nullptr) *S.status = 1;
+}
+__device__ __forceinline__ int slot_type(const Slots& S, unsigned row) {
+  const unsigned rows[1] = {row};
+  const bool in[1] = {true};
+  int t[1];
+  slot_types(S, rows, in, t);
+  return t[0] < 0 ? -1 : t[0];
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -286,6 +313,27 @@ template <class... P>
 cudaError_t allow_smem(void (*kernel)(P...), size_t bytes) {
   if (bytes <= 31 << 10) return cudaSuccess;
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+// launch_early() of blocks in clusters
+template <class... P, class... Q>
+inline cudaError_t launch_clusters(void (*kernel)(P...), unsigned blocks, unsigned cluster, unsigned threads, size_t smem, cudaStream_t st, Q... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(blocks);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  c.attrs = attr;
+  c.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
+  if (e != cudaSuccess) cudaGetLastError();  // it is in `e`: not to be found again by a later launch
+  return e;
 }
 
 // rows of which any eight columns that begin at a multiple of eight lie on 16 bytes
