@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(SortArgs A) {
 // other clusters of the launch clear the table's gradient meanwhile.  (Two launches a pass: 16384 slots of 50021 types 35 us,
 // 25551 of 350 types 16 us.)
 constexpr unsigned CLUSTER = 8, CLUSTER_KEYS = 4;
+constexpr int CLUSTER_BITS_MOST = 10;
 
 struct ClusterSortArgs {
   Slots S;
@@ -279,8 +280,8 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A
   const unsigned bins = 1u << A.bits, mask = bins - 1, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, block = blockIdx.x;
   unsigned* count = sort_shared;                                            // [bins] of this block
   unsigned* base = count + bins;                                            // [bins] first place of a digit's slots here
-  unsigned short* all = reinterpret_cast<unsigned short*>(base + bins);     // [warps][bins]
-  unsigned short* mine = all + warp * bins;
+  unsigned* all = base + bins;                                              // [warps][bins]
+  unsigned* mine = all + warp * bins;
   const unsigned per = A.each / SORT_WARPS, begin = block * A.each + warp * per, turns = begin < A.S.rows ? min(per, A.S.rows - begin) : 0;
   const unsigned lower = (1u << lane) - 1;
   for (int pass = 0; pass < A.passes; pass++) {
@@ -304,29 +305,22 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A
         row[k] = slot[k] ? __ldcg(A.row[(pass - 1) & 1] + row[k]) : 0;
       }
     }
-    for (unsigned b = lane; b < bins; b += 32) mine[b] = 0;
+    for (unsigned b = lane; b < bins / 4; b += 32) reinterpret_cast<uint4*>(mine)[b] = make_uint4(0, 0, 0, 0);
     __syncwarp();
-    unsigned peers[CLUSTER_KEYS];
 #pragma unroll
-    for (unsigned k = 0; k < CLUSTER_KEYS; k++) {
-      if (k * 32 < turns) {
-        const unsigned d = key[k] >> shift & mask;
-        peers[k] = same_digit(d, A.bits, slot[k]);
-        if (slot[k] && (peers[k] & lower) == 0) mine[d] += (unsigned short)__popc(peers[k]);
-        __syncwarp();
-      }
-    }
+    for (unsigned k = 0; k < CLUSTER_KEYS; k++)
+      if (slot[k]) atomicAdd(&mine[key[k] >> shift & mask], 1u);
     __syncthreads();
     for (unsigned b = tid; b < bins; b += SORT_THREADS) {
       unsigned at = 0;
 #pragma unroll
       for (unsigned w0 = 0; w0 < SORT_WARPS; w0 += 16) {
-        unsigned short n[16];
+        unsigned n[16];
 #pragma unroll
         for (unsigned w = 0; w < 16; w++) n[w] = all[(w0 + w) * bins + b];
 #pragma unroll
         for (unsigned w = 0; w < 16; w++) {
-          all[(w0 + w) * bins + b] = (unsigned short)at;
+          all[(w0 + w) * bins + b] = at;
           at += n[w];
         }
       }
@@ -365,9 +359,10 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A
 #pragma unroll
     for (unsigned k = 0; k < CLUSTER_KEYS; k++) {
       if (k * 32 < turns) {
-        const unsigned d = key[k] >> shift & mask, at = slot[k] ? base[d] + mine[d] + __popc(peers[k] & lower) : ~0u;
+        const unsigned d = key[k] >> shift & mask, peers = same_digit(d, A.bits, slot[k]);
+        const unsigned at = slot[k] ? base[d] + mine[d] + __popc(peers & lower) : ~0u;
         __syncwarp();
-        if (slot[k] && (peers[k] & lower) == 0) mine[d] += (unsigned short)__popc(peers[k]);
+        if (slot[k] && (peers & lower) == 0) mine[d] += __popc(peers);
         __syncwarp();
         if (at < A.S.rows) {  // always, for types that nobody changes meanwhile
           key_out[at] = key[k];
@@ -380,7 +375,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A
   }
 }
 
-size_t cluster_smem(int bits) { return (8 + 2 * SORT_WARPS) * ((size_t)1 << bits); }
+size_t cluster_smem(int bits) { return (8 + 4 * SORT_WARPS) * ((size_t)1 << bits); }
 
 size_t sort_smem(int bits) {
   const size_t bins = (size_t)1 << bits, slices = bins < SORT_THREADS ? SORT_THREADS / bins : 1;
@@ -400,24 +395,16 @@ struct PieceArgs {
 
 constexpr int PIECE_THREADS = 256, PIECE_SLOTS = 2048;  // slots of a block, at most
 
-// A group of lanes sums a piece type by type.  A type that crosses pieces is put together in shared memory by the group that it begins
-// in; only what crosses blocks is left to k_type_joins (one of a hundred pieces, so the way of a type that holds
-// many slots is short: 46 us for 25000 slots, a tenth of them of one type, without).
-template <class T, class O, bool VEC, bool DROP>
-__global__ void __launch_bounds__(PIECE_THREADS, 3) k_type_pieces(PieceArgs A, const T* diff, long long diff_ld, O* grad, long long grad_ld, Drop D) {
+// Sums of a block's sorted slots: keys[1 .. here] and rows[0 .. here - 1], keys[0] and keys[here + 1] those of the slots before and
+// behind.  A group of lanes sums a piece type by type.  A type that crosses pieces is put together in shared memory by the
+// group that it begins in; only what crosses blocks is left, in `parts` (46 us for 25000 slots, a tenth of them of one type,
+// when every piece left its own).
+template <int THREADS, class T, class O, bool VEC, bool DROP>
+__device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* keys, const unsigned* rows, float* heads, float* tails, unsigned here,
+                                           int col_tile, const T* diff, long long diff_ld, O* grad, long long grad_ld, const Drop& D, float* parts) {
   constexpr int ROWS = sizeof(T) == 2 ? 8 : 4;  // whose loads are in flight together
-  __shared__ unsigned keys[PIECE_SLOTS + 2], rows[PIECE_SLOTS];
-  __shared__ float heads[PIECE_THREADS * 8], tails[PIECE_THREADS * 8];
-  wait_for_stream();
-  const int groups = PIECE_THREADS / A.lanes, group = threadIdx.x / A.lanes, lane = threadIdx.x % A.lanes;
-  const unsigned slots = groups * A.piece, first_slot = blockIdx.x * slots, here = min(slots, A.n - first_slot);
-  for (unsigned i = threadIdx.x; i < here + 2; i += PIECE_THREADS) {
-    const unsigned at = first_slot + i;  // keys[i] is that of the slot before
-    keys[i] = at > 0 && at <= A.n ? A.key[at - 1] : ~0u;
-    if (i < here) rows[i] = A.row[at];
-  }
-  __syncthreads();
-  const int col = (blockIdx.y * A.lanes + lane) * 8;
+  const int group = threadIdx.x / A.lanes, lane = threadIdx.x % A.lanes;
+  const int col = (col_tile * A.lanes + lane) * 8;
   const unsigned begin = min(group * A.piece, here), end = min(begin + A.piece, here);
   const bool some = begin < end && col < A.width;
   const unsigned came = keys[begin], goes = keys[end + 1];
@@ -482,7 +469,6 @@ __global__ void __launch_bounds__(PIECE_THREADS, 3) k_type_pieces(PieceArgs A, c
       if (keys[last] != type || keys[last + 1] != type) return false;
     }
   };
-  float* parts = A.parts + (size_t)blockIdx.x * 2 * A.width;
   const unsigned t0 = keys[begin + 1], t1 = keys[end];
   if (group == 0 && t0 == came && t0 < A.ntypes) {
     float sum[8] = {};
@@ -496,6 +482,92 @@ __global__ void __launch_bounds__(PIECE_THREADS, 3) k_type_pieces(PieceArgs A, c
     if (follow(t1, group + 1, sum)) store_cols<float, 8, false>(parts + A.width, col, A.width, sum);
     else write(t1, sum);
   }
+}
+
+template <class T, class O, bool VEC, bool DROP>
+__global__ void __launch_bounds__(PIECE_THREADS, 3) k_type_pieces(PieceArgs A, const T* diff, long long diff_ld, O* grad, long long grad_ld, Drop D) {
+  __shared__ unsigned keys[PIECE_SLOTS + 2], rows[PIECE_SLOTS];
+  __shared__ float heads[PIECE_THREADS * 8], tails[PIECE_THREADS * 8];
+  wait_for_stream();
+  const unsigned slots = PIECE_THREADS / A.lanes * A.piece, first_slot = blockIdx.x * slots, here = min(slots, A.n - first_slot);
+  for (unsigned i = threadIdx.x; i < here + 2; i += PIECE_THREADS) {
+    const unsigned at = first_slot + i;  // keys[i] is that of the slot before
+    keys[i] = at > 0 && at <= A.n ? A.key[at - 1] : ~0u;
+    if (i < here) rows[i] = A.row[at];
+  }
+  __syncthreads();
+  sum_pieces<PIECE_THREADS, T, O, VEC, DROP>(A, keys, rows, heads, tails, here, blockIdx.y, diff, diff_ld, grad, grad_ld, D,
+                                             A.parts + (size_t)blockIdx.x * 2 * A.width);
+}
+
+// ---- up to 1024 slots, in one launch ---------------------------------------------------------------------------------------
+// The first blocks sort all slots in shared memory, (type, slot) as one word each, by bitonic merges (Batcher, "Sorting networks and their
+// applications", 1968), and sum them for 8 * lanes columns each; the others clear the rows of the types that no
+// slot has.  (Three launches otherwise: 1000 slots of 5000 types 16 us, 300 of 100000 types 14 us.)
+constexpr int SMALL_THREADS = 512, SMALL_SLOTS = 1024, SMALL_RANGE = 32768;  // types whose rows a block clears, at most
+constexpr int SMALL_TYPES = 1 << 21;
+
+template <class T, class O, bool VEC, bool DROP>
+__global__ void __launch_bounds__(SMALL_THREADS) k_type_small(Slots S, PieceArgs A, unsigned sum_blocks, unsigned range, FastDiv by_groups, const T* diff,
+                                                              long long diff_ld, O* grad, long long grad_ld, Drop D) {
+  __shared__ unsigned keys[SMALL_SLOTS + 2], rows[SMALL_SLOTS];
+  __shared__ float heads[SMALL_THREADS * 8], tails[SMALL_THREADS * 8];
+  const unsigned tid = threadIdx.x;
+  wait_for_stream();
+  const unsigned slot[2] = {tid, tid + SMALL_THREADS};
+  const bool in[2] = {slot[0] < A.n, slot[1] < A.n};
+  if (blockIdx.x >= sum_blocks) {
+    const unsigned first = (blockIdx.x - sum_blocks) * range, types = min(range, A.ntypes - first);
+    unsigned* met = reinterpret_cast<unsigned*>(heads);  // a bit a type
+    for (unsigned i = tid; i < (types + 31) / 32; i += SMALL_THREADS) met[i] = 0;
+    __syncthreads();
+    int t[2];
+    slot_types(S, slot, in, t);
+    for (int k = 0; k < 2; k++)
+      if (in[k] && t[k] >= 0 && (unsigned)t[k] - first < types) atomicOr(&met[((unsigned)t[k] - first) / 32], 1u << (((unsigned)t[k] - first) & 31));
+    __syncthreads();
+    const float zeros[8] = {};
+    const unsigned groups = by_groups.d;
+    for (unsigned i = tid; i < types * groups; i += SMALL_THREADS) {
+      const unsigned type = by_groups(i), col = (i - type * groups) * 8;
+      if (!(met[type / 32] >> (type & 31) & 1)) store_cols<O, 8, VEC>(grad + (long long)(first + type) * grad_ld, (int)col, A.width, zeros);
+    }
+    return;
+  }
+  unsigned n2 = 64;  // slots that the network sorts
+  while (n2 < A.n) n2 *= 2;
+  {
+    int t[2];
+    slot_types(S, slot, in, t);
+    for (int k = 0; k < 2; k++)
+      if (slot[k] < n2) rows[slot[k]] = in[k] ? (t[k] < 0 ? A.ntypes : (unsigned)t[k]) << 10 | slot[k] : ~0u;  // empty slots come last
+  }
+  __syncthreads();
+  for (unsigned size = 2; size <= n2; size *= 2)
+    for (unsigned stride = size / 2; stride; stride /= 2) {
+      // a warp's pairs lie in its own 64 words where they are up to 32 apart: others' are waited for at 64 and more, and behind them
+      if (stride >= 32) __syncthreads();
+      else __syncwarp();
+      if (tid < n2 / 2) {
+        const unsigned i = 2 * tid - (tid & (stride - 1)), a = rows[i], b = rows[i + stride];
+        if ((a > b) == ((i & size) == 0)) {
+          rows[i] = b;
+          rows[i + stride] = a;
+        }
+      }
+    }
+  __syncthreads();
+  unsigned word[2];
+  for (int k = 0; k < 2; k++) word[k] = in[k] ? rows[slot[k]] : 0;
+  __syncthreads();
+  for (int k = 0; k < 2; k++)
+    if (in[k]) {
+      keys[slot[k] + 1] = word[k] >> 10;
+      rows[slot[k]] = word[k] & 1023;
+    }
+  if (tid == 0) keys[0] = keys[A.n + 1] = ~0u;
+  __syncthreads();
+  sum_pieces<SMALL_THREADS, T, O, VEC, DROP>(A, keys, rows, heads, tails, A.n, blockIdx.x, diff, diff_ld, grad, grad_ld, D, nullptr);
 }
 
 // a type that begins in a block and goes on: its parts, block after block
@@ -537,7 +609,7 @@ __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* gr
 
 // ---- the plan: a function of the sizes alone, so that the workspace and the call agree ----------------------------------------
 struct Plan {
-  bool tables;
+  bool tables, small;
   // few types
   unsigned blocks, per;
   int warps;
@@ -577,11 +649,27 @@ Plan plan_for(unsigned rows, int V, int width) {
       return p;
     }
   }
+  if (rows <= SMALL_SLOTS && V < SMALL_TYPES && width <= 1 << 20) {
+    p.small = true;
+    // as many lanes as leave pieces of four slots (one round of loads), more where the blocks, which all sort, would be more than SMs
+    p.lanes = 1;
+    while (p.lanes < 32 && p.lanes * 8 < width && (rows * p.lanes * 2 <= 4 * SMALL_THREADS || width > 148 * 8 * p.lanes)) p.lanes *= 2;
+    const unsigned groups = SMALL_THREADS / p.lanes;
+    p.piece = (rows + groups - 1) / groups;
+    // blocks that clear: about 4096 groups of eight columns each, and a bit a type
+    const unsigned long long eights = (unsigned long long)V * ((width + 7) / 8);
+    unsigned blocks = (unsigned)(eights / 4096 + 1 < 1184 ? eights / 4096 + 1 : 1184);
+    if (blocks < ((unsigned)V + SMALL_RANGE - 1) / SMALL_RANGE) blocks = ((unsigned)V + SMALL_RANGE - 1) / SMALL_RANGE;
+    p.per = (V + blocks - 1) / blocks;  // types of a block
+    p.blocks = (V + p.per - 1) / p.per;
+    p.bytes = 256;
+    return p;
+  }
   int key_bits = 1, most = 1;
   while (key_bits < 31 && (unsigned)V >> key_bits) key_bits++;
   if (rows <= CLUSTER * CLUSTER_KEYS * SORT_THREADS) {
     p.tile = (rows + CLUSTER * SORT_THREADS - 1) / (CLUSTER * SORT_THREADS) * SORT_THREADS;
-    most = SORT_BITS_MOST;
+    most = CLUSTER_BITS_MOST;
   } else {
     p.tile = SORT_THREADS;
     while ((rows + p.tile - 1) / p.tile > 148 && p.tile < SORT_TILE_MOST) p.tile += SORT_THREADS;
@@ -591,6 +679,7 @@ Plan plan_for(unsigned rows, int V, int width) {
   }
   p.passes = (key_bits + most - 1) / most;
   p.bits = (key_bits + p.passes - 1) / p.passes;
+  if (p.bits < 2) p.bits = 2;
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes * 8 < width) p.lanes *= 2;
   const unsigned cols = (width + p.lanes * 8 - 1) / (p.lanes * 8);
@@ -633,6 +722,25 @@ cudaError_t by_tables(const Slots& S, const Plan& p, const lmg_vectors* diff, co
   ++*launches;
   return launch_early(k_table_sums<O>, dim3((unsigned)(((size_t)S.ntypes * width + 31) / 32)), 1024, 0, st, parts, (int)p.blocks, S.ntypes, width, g,
                       grad->ld, scale);
+}
+
+template <class T, class O>
+cudaError_t by_network(const Slots& S, const Plan& p, const lmg_vectors* diff, const lmg_vectors* grad, int width, float scale, const Drop& D,
+                       char*, long* launches, cudaStream_t st) {
+  PieceArgs P = {};
+  P.n = S.rows;
+  P.ntypes = (unsigned)S.ntypes;
+  P.piece = p.piece;
+  P.lanes = p.lanes;
+  P.width = width;
+  P.scale = scale;
+  const bool vec = rows_aligned(diff) && rows_aligned(grad);
+  const auto kernel = vec ? (drops(D) ? k_type_small<T, O, true, true> : k_type_small<T, O, true, false>)
+                          : (drops(D) ? k_type_small<T, O, false, true> : k_type_small<T, O, false, false>);
+  const unsigned sums = (width + p.lanes * 8 - 1) / (p.lanes * 8);
+  ++*launches;
+  return launch_early(kernel, dim3(sums + p.blocks), SMALL_THREADS, 0, st, S, P, sums, p.per, FastDiv((unsigned)(width + 7) / 8),
+                      static_cast<const T*>(diff->data), diff->ld, static_cast<O*>(grad->data), grad->ld, D);
 }
 
 template <class T, class O>
@@ -743,7 +851,7 @@ int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, cons
   const Drop D = to_drop(drop);
   long launches = 0;
   const cudaError_t e = by_vector_types(diff->type, table_gradients->type, [&](auto t, auto o) {
-    const auto by = p.tables ? by_tables<decltype(t), decltype(o)> : by_sort<decltype(t), decltype(o)>;
+    const auto by = p.tables ? by_tables<decltype(t), decltype(o)> : p.small ? by_network<decltype(t), decltype(o)> : by_sort<decltype(t), decltype(o)>;
     return by(S, p, diff, table_gradients, width, scale, D, static_cast<char*>(workspace), &launches, st);
   });
   lmg_internal_count_launches(launches);
