@@ -15,6 +15,22 @@ int vectors_cuda(cudaError_t e, const char* what) {
   return LMG_ERR_CUDA;
 }
 
+cudaError_t allow_smem_of(const void* kernel) {
+  struct Asked {
+    const void* kernel;
+    int device;
+  };
+  static thread_local Asked asked[64] = {};
+  int device = -1;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  Asked& a = asked[(reinterpret_cast<uintptr_t>(kernel) >> 4) % 64];
+  if (a.kernel == kernel && a.device == device) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MOST);
+  if (e == cudaSuccess) a = {kernel, device};
+  return e;
+}
+
 int check_slots(const lmg_slots* s, int width) {
   if (s == nullptr) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "null slots");
   if (s->batch < 0 || s->max_atoms < 0 || width < 0) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "negative size");

@@ -622,7 +622,7 @@ struct Plan {
   size_t key[2], row[2], counts, parts, bytes;
 };
 
-constexpr size_t TABLE_SMEM = 224 << 10;  // an SM's
+constexpr size_t TABLE_SMEM = SMEM_MOST;  // an SM's
 constexpr int TABLE_WARPS_LEAST = 4, TABLE_WARPS_MOST = 16;
 
 Plan plan_for(unsigned rows, int V, int width) {

@@ -20,8 +20,7 @@ namespace lmg {
 struct FastDiv {
   unsigned d, mul, shift;
   FastDiv() = default;
-  explicit FastDiv(unsigned by) : d(by), shift(0) {
-    while (shift < 32 && (1ull << shift) < by) shift++;
+  explicit FastDiv(unsigned by) : d(by), shift(by > 1 ? 32 - __builtin_clz(by - 1) : 0) {
     mul = (unsigned)(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
   }
 #ifdef __CUDACC__
@@ -308,11 +307,14 @@ cudaError_t by_vector_types(int in, int out, F f) {
   return f(__half(), __half());
 }
 inline size_t element_bytes(int type) { return type == LMG_FLOAT32 ? 4 : 2; }
-// more shared memory than a launch has without asking: 48 KB, its own variables among them (17 KB at most here)
+// Leave to have more shared memory than the 48 KB of any launch, its own variables among them (17 KB at most here): always for as much as
+// any launch wants, so that calls of several threads do not undo one another's, and once for each kernel and device, as far as
+// a thread remembers.
+constexpr size_t SMEM_MOST = 224 << 10;
+cudaError_t allow_smem_of(const void* kernel);
 template <class... P>
 cudaError_t allow_smem(void (*kernel)(P...), size_t bytes) {
-  if (bytes <= 31 << 10) return cudaSuccess;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return bytes <= 31 << 10 ? cudaSuccess : allow_smem_of(reinterpret_cast<const void*>(kernel));
 }
 
 // launch_early() of blocks in clusters

@@ -18,6 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _cabi
+from . import api as _api
 from . import grids as _grids
 from ._cabi import check
 from .api import _Arg, _current_device, _fast, _stream_ptr, _workspace, _workspaces
@@ -173,13 +174,8 @@ def _ref(s):
     return None if s is None else ctypes.byref(s)
 
 
-def _native_call(name, *args):
-    """The call by the compiled module, when every array is a CUDA tensor of the right kind and shape; False: the general
-    route takes it (and raises what there is to raise)."""
-    m = _fast()
-    return bool(m) and getattr(m, name)(*args) is not None
-
-
+# Each call goes to the compiled module first, which serves it when every array is a CUDA tensor of the right kind and shape, and
+# answers None when not: the general route takes those (and raises what there is to raise).
 def embed_types(types, table, out, scale=1.0, n_atoms=None, p=0.0, rng=None, status=None):
     """``out[slot] = scale * table[types[slot]]``, then dropout with probability ``p``; empty slots are zero.
 
@@ -187,7 +183,8 @@ def embed_types(types, table, out, scale=1.0, n_atoms=None, p=0.0, rng=None, sta
     table may have 16-bit outputs; otherwise the two types agree.  ``rng`` is (seed, offset), or an int64 CUDA tensor of the two, which
     the kernel reads: see :func:`dropout`.  A type >= ntypes leaves its slot empty and sets ``status``, one int32 on
     the GPU that the caller clears and reads when it suits (the check that ``GridMaker.check_types`` makes)."""
-    if _native_call("_fast_embed", types, table, out, scale, n_atoms, p, rng, status):
+    m = _api._native or _fast()
+    if m and m._fast_embed(types, table, out, scale, n_atoms, p, rng, status) is not None:
         return
     dev = _current_device()
     t, s, keep = _types(types, n_atoms, dev, status)
@@ -204,7 +201,9 @@ def embed_types(types, table, out, scale=1.0, n_atoms=None, p=0.0, rng=None, sta
 def embed_types_backward(types, diff, table_gradients, scale=1.0, n_atoms=None, p=0.0, rng=None, status=None):
     """``table_gradients[type] = scale * sum of diff[slot]`` over the type's slots, ``diff`` after the same dropout as the
     vectors; types without a slot get zero.  16-bit gradients may go into a float32 table."""
-    if _native_call("_fast_embed_backward", types, diff, table_gradients, scale, n_atoms, p, rng, status, _workspaces.by):
+    m = _api._native or _fast()
+    if m and m._fast_embed_backward(types, diff, table_gradients, scale, n_atoms, p, rng,
+            status, _workspaces.by) is not None:
         return
     dev = _current_device()
     t, s, keep = _types(types, n_atoms, dev, status)
@@ -246,7 +245,8 @@ def layer_norm(x, weight, bias, out, stats=None, eps=1e-5, n_atoms=None):
     ``x`` and ``out`` (...,W) of one type (``out`` may be ``x``), ``weight`` and ``bias`` (W,) of that type or float32, or None.
     ``n_atoms`` (B,) goes with ``x`` (B,N,W): rows behind an example's count become zero.  ``stats`` (...,2)
     float32 takes each row's mean and 1 / sqrt(variance + eps), which the backward pass reads."""
-    if _native_call("_fast_layer_norm", x, weight, bias, out, stats, eps, n_atoms):
+    m = _api._native or _fast()
+    if m and m._fast_layer_norm(x, weight, bias, out, stats, eps, n_atoms) is not None:
         return
     dev = _current_device()
     a = _Vectors(x, dev, "x")
@@ -265,8 +265,9 @@ def layer_norm(x, weight, bias, out, stats=None, eps=1e-5, n_atoms=None):
 def layer_norm_backward(x, weight, stats, diff, x_gradients, weight_gradients=None, bias_gradients=None, n_atoms=None):
     """Gradients of :func:`layer_norm` from ``diff``, that of its output, and the ``stats`` it filled.  ``x_gradients`` may
     be ``diff``; gradients of weights or biases that are not wanted are None."""
-    if _native_call("_fast_layer_norm_backward", x, weight, stats, diff, x_gradients, weight_gradients, bias_gradients, n_atoms,
-                    _workspaces.by):
+    m = _api._native or _fast()
+    if m and m._fast_layer_norm_backward(x, weight, stats, diff, x_gradients, weight_gradients,
+            bias_gradients, n_atoms, _workspaces.by) is not None:
         return
     dev = _current_device()
     a = _Vectors(x, dev, "x")
@@ -295,7 +296,8 @@ def dropout(x, out, p, rng):
     row (all leading dimensions taken in order) and its column alone, so the gradient is the same call on the gradient.
     ``rng`` is (seed, offset) - another offset for each draw - or an int64 CUDA tensor of the two, which the kernel reads
     (:func:`next_draw` takes it from a generator state on the GPU: the form for calls that are captured and replayed)."""
-    if _native_call("_fast_dropout", x, out, p, rng):
+    m = _api._native or _fast()
+    if m and m._fast_dropout(x, out, p, rng) is not None:
         return
     dev = _current_device()
     a = _Vectors(x, dev, "x")
