@@ -395,28 +395,70 @@ struct PieceArgs {
 
 constexpr int PIECE_THREADS = 256, PIECE_SLOTS = 2048;  // slots of a block, at most
 
+// The eight columns of a lane: next to each other where rows lie on 16 bytes, else every `lanes`th, so that neighbouring lanes touch
+// neighbouring values (61 slots of 1402 types, 231 float32: 16 us with eight single values a lane next to each other).
+template <bool VEC>
+struct Columns {
+  int first, step, width;
+  __device__ __forceinline__ Columns(int tile, int lane, int lanes, int width_)
+      : first(VEC ? (tile * lanes + lane) * 8 : tile * lanes * 8 + lane), step(VEC ? 1 : lanes), width(width_) {}
+  __device__ __forceinline__ bool any() const { return first < width; }
+  template <class T>
+  __device__ __forceinline__ void store(T* row, const float (&v)[8]) const {
+    if constexpr (VEC) {
+      store_cols<T, 8, true>(row, first, width, v);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 8; c++)
+        if (first + c * step < width) row[first + c * step] = from_float<T>(v[c]);
+    }
+  }
+  __device__ __forceinline__ void load(const float* row, float (&v)[8]) const {  // of partial sums, which lie anywhere
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = first + c * step < width ? row[first + c * step] : 0.f;
+  }
+};
+template <class T, bool VEC>
+struct PieceRow {
+  Raw<T, 8, true> raw;
+  __device__ __forceinline__ void load(const T* row, const Columns<VEC>& C) { raw.load(row, C.first, C.width); }
+  __device__ __forceinline__ float get(int c) const { return raw.get(c); }
+};
+template <class T>
+struct PieceRow<T, false> {
+  T v[8];
+  __device__ __forceinline__ void load(const T* row, const Columns<false>& C) {
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = C.first + c * C.step < C.width ? row[C.first + c * C.step] : from_float<T>(0.f);
+  }
+  __device__ __forceinline__ float get(int c) const { return to_float(v[c]); }
+};
+
 // Sums of a block's sorted slots: keys[1 .. here] and rows[0 .. here - 1], keys[0] and keys[here + 1] those of the slots before and
 // behind.  A group of lanes sums a piece type by type.  A type that crosses pieces is put together in shared memory by the
 // group that it begins in; only what crosses blocks is left, in `parts` (46 us for 25000 slots, a tenth of them of one type,
 // when every piece left its own).
-template <int THREADS, class T, class O, bool VEC, bool DROP>
+template <class T, class O, bool VEC, bool DROP>
 __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* keys, const unsigned* rows, float* heads, float* tails, unsigned here,
                                            int col_tile, const T* diff, long long diff_ld, O* grad, long long grad_ld, const Drop& D, float* parts) {
-  constexpr int ROWS = sizeof(T) == 2 ? 8 : 4;  // whose loads are in flight together
+  constexpr int ROWS = VEC && sizeof(T) == 2 ? 8 : 4;  // whose loads are in flight together
   const int group = threadIdx.x / A.lanes, lane = threadIdx.x % A.lanes;
-  const int col = (col_tile * A.lanes + lane) * 8;
+  const Columns<VEC> C(col_tile, lane, A.lanes, A.width);
   const unsigned begin = min(group * A.piece, here), end = min(begin + A.piece, here);
-  const bool some = begin < end && col < A.width;
+  const bool some = begin < end && C.any();
   const unsigned came = keys[begin], goes = keys[end + 1];
   float* head = heads + (size_t)group * A.lanes * 8 + lane * 8;
   float* tail = tails + (size_t)group * A.lanes * 8 + lane * 8;
   auto write = [&](unsigned type, float (&sum)[8]) {
 #pragma unroll
     for (int c = 0; c < 8; c++) sum[c] *= A.scale;
-    store_cols<O, 8, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
+    C.store(grad + (long long)type * grad_ld, sum);
   };
   if (some) {
     const DropKey K(D);
+    // a group's lanes that are at work, and where in the warp it begins: they hand their bits round
+    const int left = A.width - col_tile * A.lanes * 8, first_lane = (threadIdx.x & 31) - lane;
+    const unsigned together = (left >= 32 ? ~0u : (1u << min(left, A.lanes)) - 1) >> (left >= 32 ? 32 - A.lanes : 0) << first_lane;
     float sum[8] = {};
     unsigned type = keys[begin + 1];
     bool first = true;
@@ -433,10 +475,10 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
       }
     };
     for (unsigned i = begin; i < end; i += ROWS) {
-      Raw<T, 8, VEC> v[ROWS];
+      PieceRow<T, VEC> v[ROWS];
 #pragma unroll
       for (int j = 0; j < ROWS; j++)
-        if (i + j < end && keys[i + j + 1] < A.ntypes) v[j].load(diff + (long long)rows[i + j] * diff_ld, col, A.width);
+        if (i + j < end && keys[i + j + 1] < A.ntypes) v[j].load(diff + (long long)rows[i + j] * diff_ld, C);
 #pragma unroll
       for (int j = 0; j < ROWS; j++) {
         if (i + j >= end) break;
@@ -449,9 +491,18 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
           for (int c = 0; c < 8; c++) sum[c] = 0.f;
         }
         if (type >= A.ntypes) continue;
-        const unsigned keep = DROP ? kept8(D, K, rows[i + j], col / 8) : 0xff;
+        if (DROP) {
+          const unsigned bits = kept8(D, K, rows[i + j], col_tile * A.lanes + lane);
 #pragma unroll
-        for (int c = 0; c < 8; c++) sum[c] += DROP ? (keep >> c & 1 ? v[j].get(c) * D.scale : 0.f) : v[j].get(c);
+          for (int c = 0; c < 8; c++) {
+            const int at = lane + c * A.lanes;  // of the tile's columns
+            const bool stays = VEC ? bits >> c & 1 : __shfl_sync(together, bits, first_lane + at / 8) >> (at & 7) & 1;
+            sum[c] += stays ? v[j].get(c) * D.scale : 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; c++) sum[c] += v[j].get(c);
+        }
       }
     }
     put(true);
@@ -469,23 +520,28 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
       if (keys[last] != type || keys[last + 1] != type) return false;
     }
   };
+  auto put_part = [&](float* to, const float (&sum)[8]) {
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+      if (C.first + c * C.step < A.width) to[C.first + c * C.step] = sum[c];
+  };
   const unsigned t0 = keys[begin + 1], t1 = keys[end];
   if (group == 0 && t0 == came && t0 < A.ntypes) {
     float sum[8] = {};
     follow(t0, 0, sum);
-    store_cols<float, 8, false>(parts, col, A.width, sum);
+    put_part(parts, sum);
   }
   if (goes == t1 && t1 < A.ntypes && !(t0 == t1 && came == t0)) {
     float sum[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) sum[c] = tail[c];
-    if (follow(t1, group + 1, sum)) store_cols<float, 8, false>(parts + A.width, col, A.width, sum);
+    if (follow(t1, group + 1, sum)) put_part(parts + A.width, sum);
     else write(t1, sum);
   }
 }
 
 template <class T, class O, bool VEC, bool DROP>
-__global__ void __launch_bounds__(PIECE_THREADS, 3) k_type_pieces(PieceArgs A, const T* diff, long long diff_ld, O* grad, long long grad_ld, Drop D) {
+__global__ void __launch_bounds__(PIECE_THREADS, DROP ? 2 : 3) k_type_pieces(PieceArgs A, const T* diff, long long diff_ld, O* grad, long long grad_ld, Drop D) {
   __shared__ unsigned keys[PIECE_SLOTS + 2], rows[PIECE_SLOTS];
   __shared__ float heads[PIECE_THREADS * 8], tails[PIECE_THREADS * 8];
   wait_for_stream();
@@ -496,7 +552,7 @@ __global__ void __launch_bounds__(PIECE_THREADS, 3) k_type_pieces(PieceArgs A, c
     if (i < here) rows[i] = A.row[at];
   }
   __syncthreads();
-  sum_pieces<PIECE_THREADS, T, O, VEC, DROP>(A, keys, rows, heads, tails, here, blockIdx.y, diff, diff_ld, grad, grad_ld, D,
+  sum_pieces<T, O, VEC, DROP>(A, keys, rows, heads, tails, here, blockIdx.y, diff, diff_ld, grad, grad_ld, D,
                                              A.parts + (size_t)blockIdx.x * 2 * A.width);
 }
 
@@ -508,7 +564,7 @@ constexpr int SMALL_THREADS = 512, SMALL_SLOTS = 1024, SMALL_RANGE = 32768;  // 
 constexpr int SMALL_TYPES = 1 << 21;
 
 template <class T, class O, bool VEC, bool DROP>
-__global__ void __launch_bounds__(SMALL_THREADS) k_type_small(Slots S, PieceArgs A, unsigned sum_blocks, unsigned range, FastDiv by_groups, const T* diff,
+__global__ void __launch_bounds__(SMALL_THREADS) k_type_small(Slots S, PieceArgs A, unsigned sum_blocks, unsigned range, FastDiv by_units, const T* diff,
                                                               long long diff_ld, O* grad, long long grad_ld, Drop D) {
   __shared__ unsigned keys[SMALL_SLOTS + 2], rows[SMALL_SLOTS];
   __shared__ float heads[SMALL_THREADS * 8], tails[SMALL_THREADS * 8];
@@ -526,11 +582,18 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_type_small(Slots S, PieceArgs
     for (int k = 0; k < 2; k++)
       if (in[k] && t[k] >= 0 && (unsigned)t[k] - first < types) atomicOr(&met[((unsigned)t[k] - first) / 32], 1u << (((unsigned)t[k] - first) & 31));
     __syncthreads();
-    const float zeros[8] = {};
-    const unsigned groups = by_groups.d;
-    for (unsigned i = tid; i < types * groups; i += SMALL_THREADS) {
-      const unsigned type = by_groups(i), col = (i - type * groups) * 8;
-      if (!(met[type / 32] >> (type & 31) & 1)) store_cols<O, 8, VEC>(grad + (long long)(first + type) * grad_ld, (int)col, A.width, zeros);
+    // eight values a thread and turn where rows lie on 16 bytes, else one, by columns
+    const unsigned units = by_units.d;
+    for (unsigned i = tid; i < types * units; i += SMALL_THREADS) {
+      const unsigned type = by_units(i), at = i - type * units;
+      if (met[type / 32] >> (type & 31) & 1) continue;
+      O* row = grad + (long long)(first + type) * grad_ld;
+      if constexpr (VEC) {
+        const float zeros[8] = {};
+        store_cols<O, 8, true>(row, (int)at * 8, A.width, zeros);
+      } else {
+        row[at] = from_float<O>(0.f);
+      }
     }
     return;
   }
@@ -567,7 +630,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_type_small(Slots S, PieceArgs
     }
   if (tid == 0) keys[0] = keys[A.n + 1] = ~0u;
   __syncthreads();
-  sum_pieces<SMALL_THREADS, T, O, VEC, DROP>(A, keys, rows, heads, tails, A.n, blockIdx.x, diff, diff_ld, grad, grad_ld, D, nullptr);
+  sum_pieces<T, O, VEC, DROP>(A, keys, rows, heads, tails, A.n, blockIdx.x, diff, diff_ld, grad, grad_ld, D, nullptr);
 }
 
 // a type that begins in a block and goes on: its parts, block after block
@@ -575,14 +638,14 @@ template <class O, bool VEC>
 __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* grad, long long grad_ld) {
   wait_for_stream();
   const unsigned at = blockIdx.x * PIECE_THREADS + threadIdx.x, block = at / A.lanes, slots = PIECE_THREADS / A.lanes * A.piece;
-  const int col = (blockIdx.y * A.lanes + at % A.lanes) * 8;
-  if (block + 1 >= A.blocks || col >= A.width) return;
+  const Columns<VEC> C(blockIdx.y, at % A.lanes, A.lanes, A.width);
+  if (block + 1 >= A.blocks || !C.any()) return;
   // all that a type which ends in the next block needs is on its way before it is known whether there is one
   const unsigned begin = block * slots, end = begin + slots, type = A.key[end - 1], goes = A.key[end], came = begin > 0 ? A.key[begin - 1] : ~0u;
   const unsigned after = block + 2 < A.blocks ? A.key[end + slots] : ~0u;
   float sum[8], more[8];
-  load_cols<float, 8, false>(A.parts + ((size_t)block * 2 + 1) * A.width, col, A.width, sum);
-  load_cols<float, 8, false>(A.parts + ((size_t)block + 1) * 2 * A.width, col, A.width, more);
+  C.load(A.parts + ((size_t)block * 2 + 1) * A.width, sum);
+  C.load(A.parts + ((size_t)block + 1) * 2 * A.width, more);
   if (type >= A.ntypes || goes != type || came == type) return;
 #pragma unroll
   for (int c = 0; c < 8; c++) sum[c] += more[c];
@@ -590,7 +653,7 @@ __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* gr
   while (p + 4 <= A.blocks && A.key[(p + 3) * slots] == type) {
     float v[4][8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) load_cols<float, 8, false>(A.parts + (size_t)(p + j) * 2 * A.width, col, A.width, v[j]);
+    for (int j = 0; j < 4; j++) C.load(A.parts + (size_t)(p + j) * 2 * A.width, v[j]);
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -598,13 +661,13 @@ __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* gr
     p += 4;
   }
   for (; p < A.blocks && A.key[p * slots] == type; p++) {
-    load_cols<float, 8, false>(A.parts + (size_t)p * 2 * A.width, col, A.width, more);
+    C.load(A.parts + (size_t)p * 2 * A.width, more);
 #pragma unroll
     for (int c = 0; c < 8; c++) sum[c] += more[c];
   }
 #pragma unroll
   for (int c = 0; c < 8; c++) sum[c] *= A.scale;
-  store_cols<O, 8, VEC>(grad + (long long)type * grad_ld, col, A.width, sum);
+  C.store(grad + (long long)type * grad_ld, sum);
 }
 
 // ---- the plan: a function of the sizes alone, so that the workspace and the call agree ----------------------------------------
@@ -624,6 +687,9 @@ struct Plan {
 
 constexpr size_t TABLE_SMEM = SMEM_MOST;  // an SM's
 constexpr int TABLE_WARPS_LEAST = 4, TABLE_WARPS_MOST = 16;
+// Tiles of 32 columns, and slots times tiles, up to which tables are kept: 200000 slots of 28 types and 128 float32 take 45.5 us with them
+// and 46.5 sorted, of 256 bfloat16 78 and 64, 20000 of 200 float32 10.6 and 23.5.
+constexpr unsigned TABLE_TILES = 8, TABLE_WORK = 1 << 20;
 
 Plan plan_for(unsigned rows, int V, int width) {
   Plan p = {};
@@ -633,7 +699,8 @@ Plan plan_for(unsigned rows, int V, int width) {
   }
   // tables: four a warp; fewer than four warps an SM have too few loads in flight
   const size_t warp_smem = (size_t)4 * V * TABLE_COLS * 4;
-  if (warp_smem * TABLE_WARPS_LEAST <= TABLE_SMEM) {
+  const unsigned col_tiles = ((unsigned)width + TABLE_COLS - 1) / TABLE_COLS;
+  if (warp_smem * TABLE_WARPS_LEAST <= TABLE_SMEM && col_tiles <= TABLE_TILES && (size_t)rows * col_tiles <= TABLE_WORK) {
     p.warps = (int)(TABLE_SMEM / warp_smem < TABLE_WARPS_MOST ? TABLE_SMEM / warp_smem : TABLE_WARPS_MOST);
     const unsigned all = (rows + 31) / 32;  // warps that find 32 slots
     if (all < 148u * p.warps) p.warps = all / 148 < TABLE_WARPS_LEAST ? TABLE_WARPS_LEAST : (int)(all / 148);
@@ -656,9 +723,9 @@ Plan plan_for(unsigned rows, int V, int width) {
     while (p.lanes < 32 && p.lanes * 8 < width && (rows * p.lanes * 2 <= 4 * SMALL_THREADS || width > 148 * 8 * p.lanes)) p.lanes *= 2;
     const unsigned groups = SMALL_THREADS / p.lanes;
     p.piece = (rows + groups - 1) / groups;
-    // blocks that clear: about 4096 groups of eight columns each, and a bit a type
+    // blocks that clear: about 512 groups of eight columns each, and a bit a type
     const unsigned long long eights = (unsigned long long)V * ((width + 7) / 8);
-    unsigned blocks = (unsigned)(eights / 4096 + 1 < 1184 ? eights / 4096 + 1 : 1184);
+    unsigned blocks = (unsigned)(eights / 512 + 1 < 592 ? eights / 512 + 1 : 592);
     if (blocks < ((unsigned)V + SMALL_RANGE - 1) / SMALL_RANGE) blocks = ((unsigned)V + SMALL_RANGE - 1) / SMALL_RANGE;
     p.per = (V + blocks - 1) / blocks;  // types of a block
     p.blocks = (V + p.per - 1) / p.per;
@@ -739,7 +806,7 @@ cudaError_t by_network(const Slots& S, const Plan& p, const lmg_vectors* diff, c
                           : (drops(D) ? k_type_small<T, O, false, true> : k_type_small<T, O, false, false>);
   const unsigned sums = (width + p.lanes * 8 - 1) / (p.lanes * 8);
   ++*launches;
-  return launch_early(kernel, dim3(sums + p.blocks), SMALL_THREADS, 0, st, S, P, sums, p.per, FastDiv((unsigned)(width + 7) / 8),
+  return launch_early(kernel, dim3(sums + p.blocks), SMALL_THREADS, 0, st, S, P, sums, p.per, FastDiv(vec ? (unsigned)(width + 7) / 8 : (unsigned)width),
                       static_cast<const T*>(diff->data), diff->ld, static_cast<O*>(grad->data), grad->ld, D);
 }
 
