@@ -279,7 +279,7 @@ int lmg_sum_types(const float* type_index, const float* type_vector, int n, int 
  * Vectors are float32, bfloat16 or float16; every product and sum is float32 and a result is rounded
  * once.  Which kernels a call takes, and with them the last bits of its sums, goes by its sizes and types and by the alignment of its
  * arrays; the same call has the same bits again.  A row has unit stride inside, rows lie `ld` elements apart (ld >= width); elements between
- * rows are not written.  Outputs may not overlap inputs, except where a comment allows it. */
+ * rows are not written.  Rows have fewer than 2^30 values, those of table gradients up to 2^23.  Outputs may not overlap inputs, except where a comment allows it. */
 enum { LMG_FLOAT32 = 0, LMG_BFLOAT16 = 1, LMG_FLOAT16 = 2 }; /* of vectors */
 enum { LMG_INDEX_FLOAT32 = 0, LMG_INDEX_INT32 = 1, LMG_INDEX_INT64 = 2 }; /* of type indices */
 

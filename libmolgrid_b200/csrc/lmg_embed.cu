@@ -35,6 +35,7 @@ int check_slots(const lmg_slots* s, int width) {
   if (s == nullptr) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "null slots");
   if (s->batch < 0 || s->max_atoms < 0 || width < 0) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "negative size");
   if ((long long)s->batch * s->max_atoms >= 0x7fffffffll) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "2^31 slots and more");
+  if (width >= 1 << 30) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "2^30 columns and more");
   return LMG_OK;
 }
 
@@ -167,39 +168,51 @@ __global__ void __launch_bounds__(256, 6) k_rows_aligned(RowArgs A, const T* src
   }
 }
 
-// Rows of any width that follow one another without gaps, from 16 bytes on: a block writes 2048 values, 16 bytes a thread and
+// Rows of any width that follow one another without gaps, from 16 bytes on: a block writes eight values a thread, 16 bytes a thread and
 // turn (with 4 bytes 8476 looked up rows of 3005 bfloat16 take 61 us instead of 54), wherever rows begin and end in them.  The types of its rows, and which of its values stay, a bit each, are made once,
 // in shared memory.
-constexpr int FLAT = 2048;
-
-template <class T, class O, bool LOOKUP, bool DROP>
-__global__ void __launch_bounds__(256, 6) k_rows_flat(RowArgs A, const T* src, O* out) {
+template <class T, class O, bool LOOKUP, bool DROP, int THREADS>
+__global__ void __launch_bounds__(THREADS, (DROP ? 1280 : 1536) / THREADS) k_rows_flat(RowArgs A, const T* src, O* out) {
+  constexpr int FLAT = 8 * THREADS;
   __shared__ unsigned kept[DROP ? FLAT / 32 : 1];
   __shared__ int types[LOOKUP ? FLAT : 1];
   const unsigned n = A.rows * (unsigned)A.width, e0 = blockIdx.x * FLAT, end = min(e0 + FLAT, n);
   const unsigned row0 = A.by_width(e0), row1 = A.by_width(end - 1), groups = A.by_groups.d;
   if (DROP) {
-    for (int i = threadIdx.x; i < FLAT / 32; i += 256) kept[i] = 0;
+    for (int i = threadIdx.x; i < FLAT / 32; i += THREADS) kept[i] = 0;
     __syncthreads();
   }
   wait_for_stream();
-  constexpr int N = 16 / (int)sizeof(O), TURNS = FLAT / 256 / N;
+  constexpr int N = 16 / (int)sizeof(O), TURNS = 8 / N;
   const T* from = src + (LOOKUP ? 0 : (long long)A.first * A.width);
   O* to = out + (long long)A.first * A.width;
   Raw<T, LOOKUP ? 4 : N> raw[LOOKUP ? 1 : TURNS];  // on their way while the bits are made
   if constexpr (!LOOKUP) {
 #pragma unroll
     for (int j = 0; j < TURNS; j++) {
-      const unsigned e = e0 + (j * 256 + threadIdx.x) * N;
+      const unsigned e = e0 + (j * THREADS + threadIdx.x) * N;
       if (e < end) raw[j].load(from + e, 0, (int)min(end - e, (unsigned)N));
     }
   }
   if (LOOKUP)
-    for (unsigned r = row0 + threadIdx.x; r <= row1; r += 256) types[r - row0] = slot_type(A.S, A.first + r);
+    for (unsigned r0 = row0 + threadIdx.x; r0 <= row1; r0 += 4 * THREADS) {  // four at a time are on their way
+      unsigned r[4];
+      bool in[4];
+      int t[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        r[k] = A.first + r0 + k * THREADS;
+        in[k] = r0 + k * THREADS <= row1;
+      }
+      slot_types(A.S, r, in, t);
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (in[k]) types[r0 + k * THREADS - row0] = t[k];
+    }
   if (DROP) {
     const DropKey K(A.D);
     const unsigned g0 = row0 * groups + (e0 - row0 * A.width) / 8, g1 = row1 * groups + (end - 1 - row1 * A.width) / 8;
-    for (unsigned g = g0 + threadIdx.x; g <= g1; g += 256) {
+    for (unsigned g = g0 + threadIdx.x; g <= g1; g += THREADS) {
       const unsigned r = A.by_groups(g), in_row = g - r * groups;
       unsigned bits = kept8(A.D, K, A.first + r, in_row);
       if ((in_row + 1) * 8 > (unsigned)A.width) bits &= (1u << (A.width & 7)) - 1;
@@ -214,7 +227,7 @@ __global__ void __launch_bounds__(256, 6) k_rows_flat(RowArgs A, const T* src, O
   if (LOOKUP || DROP) __syncthreads();
 #pragma unroll
   for (int j = 0; j < TURNS; j++) {
-    const unsigned e = e0 + (j * 256 + threadIdx.x) * N;
+    const unsigned e = e0 + (j * THREADS + threadIdx.x) * N;
     if (e >= end) break;
     const bool whole = e + N <= end;
     float v[N];
@@ -288,7 +301,7 @@ cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vector
                     (LOOKUP || (src->ld == width && reinterpret_cast<uintptr_t>(src->data) % 16 == 0));
   // passes of less than 2^30 values, a multiple of eight rows so that each begins on 16 bytes again
   const unsigned most = width > 1 << 26 ? 0 : (1u << 30) / (unsigned)width & ~7u;
-  return by_vector_types(src->type, out->type, [&](auto t, auto o) {
+  return by_vector_types<LOOKUP, false>(src->type, out->type, [&](auto t, auto o) {
     typedef decltype(t) T;
     typedef decltype(o) O;
     const T* from = static_cast<const T*>(src->data);
@@ -303,8 +316,12 @@ cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vector
       A.rows = S.rows - A.first < most ? S.rows - A.first : most;
       ++*launches;
       if (!aligned) {
-        e = launch_early(drops(D) ? k_rows_flat<T, O, LOOKUP, true> : k_rows_flat<T, O, LOOKUP, false>,
-                         dim3((unsigned)(((long long)A.rows * width + FLAT - 1) / FLAT)), 256, 0, st, A, from, to);
+        // few values: more blocks of fewer threads, which wait for fewer draws
+        const long long n = (long long)A.rows * width;
+        const int threads = n <= 148 * 2048 ? 64 : 256;
+        auto kernel = drops(D) ? k_rows_flat<T, O, LOOKUP, true, 256> : k_rows_flat<T, O, LOOKUP, false, 256>;
+        if (threads == 64) kernel = drops(D) ? k_rows_flat<T, O, LOOKUP, true, 64> : k_rows_flat<T, O, LOOKUP, false, 64>;
+        e = launch_early(kernel, dim3((unsigned)((n + 8 * threads - 1) / (8 * threads))), threads, 0, st, A, from, to);
         continue;
       }
       // 16 bytes a thread of whatever is wider; dropout goes by eights

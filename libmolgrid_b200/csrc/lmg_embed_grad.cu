@@ -899,6 +899,7 @@ int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, cons
   using namespace lmg;
   int rc;
   if ((rc = check_slots(slots, width)) || (rc = check_index(slots, ntypes)) || (rc = check_drop(drop))) return rc;
+  if (width > 1 << 23) return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "table gradients of more than 2^23 columns");
   if (ntypes == 0 || width == 0) return LMG_OK;
   if ((rc = check_vectors(table_gradients, width, "table gradients"))) return rc;
   const bool none = slots->batch == 0 || slots->max_atoms == 0;
@@ -917,7 +918,7 @@ int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, cons
   }
   const Drop D = to_drop(drop);
   long launches = 0;
-  const cudaError_t e = by_vector_types(diff->type, table_gradients->type, [&](auto t, auto o) {
+  const cudaError_t e = by_vector_types<false, true>(diff->type, table_gradients->type, [&](auto t, auto o) {
     const auto by = p.tables ? by_tables<decltype(t), decltype(o)> : p.small ? by_network<decltype(t), decltype(o)> : by_sort<decltype(t), decltype(o)>;
     return by(S, p, diff, table_gradients, width, scale, D, static_cast<char*>(workspace), &launches, st);
   });

@@ -295,14 +295,19 @@ Slots to_slots(const lmg_slots* s, int ntypes);
 Drop to_drop(const lmg_dropout_spec* d);  // upper and lower 0: nothing is dropped
 inline bool drops(const Drop& D) { return D.upper != 0 || D.lower != 0; }
 size_t embed_backward_bytes(unsigned rows, int ntypes, int width);
-// f(T, O) for the element types of source and result, which agree or are float32 and 16 bits
-template <class F>
+// f(T, O) for the element types of source and result, which agree or are float32 and 16 bits: NARROW, a float32 source of 16-bit results;
+// WIDEN, the other way round
+template <bool NARROW, bool WIDEN, class F>
 cudaError_t by_vector_types(int in, int out, F f) {
-  if (in == LMG_FLOAT32 && out == LMG_FLOAT32) return f(float(), float());
-  if (in == LMG_FLOAT32 && out == LMG_BFLOAT16) return f(float(), __nv_bfloat16());
-  if (in == LMG_FLOAT32 && out == LMG_FLOAT16) return f(float(), __half());
-  if (in == LMG_BFLOAT16 && out == LMG_FLOAT32) return f(__nv_bfloat16(), float());
-  if (in == LMG_FLOAT16 && out == LMG_FLOAT32) return f(__half(), float());
+  if constexpr (NARROW) {
+    if (in == LMG_FLOAT32 && out == LMG_BFLOAT16) return f(float(), __nv_bfloat16());
+    if (in == LMG_FLOAT32 && out == LMG_FLOAT16) return f(float(), __half());
+  }
+  if constexpr (WIDEN) {
+    if (in == LMG_BFLOAT16 && out == LMG_FLOAT32) return f(__nv_bfloat16(), float());
+    if (in == LMG_FLOAT16 && out == LMG_FLOAT32) return f(__half(), float());
+  }
+  if (in == LMG_FLOAT32) return f(float(), float());
   if (in == LMG_BFLOAT16) return f(__nv_bfloat16(), __nv_bfloat16());
   return f(__half(), __half());
 }

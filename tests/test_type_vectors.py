@@ -40,6 +40,7 @@ def test_lookup_refusals(lib):
     refused(lib, call(V=-1), "negative size")
     refused(lib, call(W=-4), "negative size")
     refused(lib, call(slots(1 << 16, 1 << 15)), "2^31 slots")
+    refused(lib, call(W=1 << 30, table=vec(1 << 30), out=vec(1 << 30)), "2^30 columns")
     refused(lib, call(slots(index=None)), "type indices missing memory")
     refused(lib, call(slots(kind=3)), "unknown element type")
     refused(lib, call(table=vec(3)), "rows overlap")
@@ -57,6 +58,8 @@ def test_lookup_refusals(lib):
 def test_gradient_refusals(lib):
     def call(s=None, V=5, W=4, diff=None, grad=None, ws=P, nbytes=1 << 40):
         return lib.lmg_embed_types_backward(s or slots(), V, W, diff or vec(4), 1.0, None, grad or vec(4), ws, nbytes, None)
+    refused(lib, call(W=(1 << 23) + 1, diff=vec(1 << 24), grad=vec(1 << 24)), "2^23 columns")
+    refused(lib, call(ws=P + 8), "off 16 bytes", _cabi.LMG_ERR_WORKSPACE)
     refused(lib, call(grad=vec(4, _cabi.FLOAT16)), "differ in type")
     refused(lib, call(diff=vec(4, _cabi.FLOAT16), grad=vec(4, _cabi.BFLOAT16)), "differ in type")
     refused(lib, call(ws=None), "workspace too small", _cabi.LMG_ERR_WORKSPACE)
@@ -79,6 +82,8 @@ def test_norm_refusals(lib):
         return lib.lmg_layer_norm_backward(slots(), 4, x or vec(4), None, wtype, stats, diff or vec(4), grad or vec(4), None, None, ws,
                                            nbytes, None)
     refused(lib, back(stats=None), "stats missing")
+    refused(lib, back(stats=P + 4), "not aligned to 8")
+    refused(lib, back(ws=P + 8), "off 16 bytes", _cabi.LMG_ERR_WORKSPACE)
     refused(lib, back(diff=vec(4, _cabi.FLOAT16)), "differ in type")
     refused(lib, back(grad=vec(2)), "rows overlap")
     refused(lib, back(ws=None), "workspace too small", _cabi.LMG_ERR_WORKSPACE)

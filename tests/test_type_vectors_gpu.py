@@ -90,6 +90,13 @@ LOOKUPS = [
     ((20000,), 20000, 13, H, H, torch.int64, 0.3, 0, 0),
     ((30000,), 70001, 16, F, F, torch.int64, 0.3, 0, 0),
     ((128, 500), 90, 31, F, F, F, 0.0, 0, 0),
+    # sorted in several launches
+    ((40000,), 5000, 24, F, F, torch.int64, 0.2, 0, 0), ((33000,), 70001, 9, H, H, torch.int64, 0.1, 0, 0),
+    ((10, 4500), 1500, 12, F, B, F, 0.0, 4, 0), ((32769,), 130, 40, F, F, torch.int32, 0.3, 0, 1),
+    # few types of wide rows, which are sorted too; one slot more than a network sorts, and as many as it does
+    ((3000,), 30, 300, F, F, F, 0.0, 0, 0), ((700,), 20, 1000, B, B, F, 0.3, 0, 0), ((1025,), 4000, 20, F, F, torch.int32, 0.0, 0, 0),
+    ((1024,), 4000, 21, F, F, torch.int32, 0.4, 0, 0), ((1024,), 2097151, 4, F, F, torch.int32, 0.0, 0, 0),
+    ((900,), 2097152, 4, F, F, torch.int32, 0.0, 0, 0), ((32768,), 113, 16, F, F, torch.int32, 0.0, 0, 0),
 ]
 IDS = ["%s-%dx%d-%s" % ("x".join(map(str, c[0])), c[1], c[2], str(c[4])[6:]) for c in LOOKUPS]
 
@@ -191,6 +198,8 @@ NORMS = [
     ((300,), 128, F, F, 4, 4), ((2, 60), 333, F, F, 0, 0), ((130,), 512, B, F, 0, 0), ((2, 60), 1001, H, H, 0, 0), ((130,), 1024, F, F, 0, 0),
     ((2, 33), 2050, B, F, 0, 0), ((33,), 4096, B, F, 0, 0), ((9,), 8192, F, F, 0, 0), ((9,), 8200, H, H, 0, 0), ((5,), 16391, F, F, 0, 0),
     ((3,), 40000, B, B, 0, 0), ((20000,), 8, F, F, 0, 0), ((3000,), 257, B, F, 0, 0), ((50000,), 28, F, F, 0, 0), ((4000,), 1032, H, F, 0, 0),
+    ((700,), 505, H, H, 0, 0), ((300,), 511, F, F, 1, 1), ((2100,), 17, B, B, 0, 0), ((640,), 64, F, F, 0, 0), ((640,), 65, F, F, 0, 0),
+    ((1300,), 2048, B, B, 0, 0), ((900,), 5984, B, F, 0, 0), ((170,), 8191, F, F, 0, 0), ((170,), 8185, H, H, 0, 1), ((2000,), 700, H, F, 0, 0),
 ]
 
 
