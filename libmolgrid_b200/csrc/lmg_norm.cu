@@ -390,9 +390,11 @@ __global__ void __maxnreg__(VALUES == 16 ? 128 : 80) k_norm_backward(NormArgs A,
   // The block's sums by way of the ring, so that neighbouring threads write neighbouring columns (each thread its own columns: 690 rows of 5984
   // bfloat16 22.8 us instead of 16.8); or the call's, where one block does all.
   float* all = reinterpret_cast<float*>(ring);
-  auto place = [&](int which, int r, int c) -> float& {  // a column's place, a word more every 32
-    const int at = (which * (int)rows + r) * A.width + c;
-    return all[at + at / 32];
+  // a column's place: a word more every 32, or rows of an odd pitch, for which no division is needed; rows that no thread has had are left out
+  const int used = min((int)rows, (int)A.S.rows), pitch = A.width | 1;
+  auto place = [&](int which, int r, int c) -> float& {
+    const int at = SPAN ? which * A.width + c : (which * used + r) * pitch + c;
+    return all[SPAN ? at + at / 32 : at];
   };
   auto put = [&](int which, int c, float v) {
     if (gridDim.x > 1) {
@@ -410,7 +412,7 @@ __global__ void __maxnreg__(VALUES == 16 ? 128 : 80) k_norm_backward(NormArgs A,
     split(db[i / 2], f[2], f[3]);
 #pragma unroll
     for (int k = 0; k < 4; k++)
-      if (share.valid(i + k % 2)) place(k / 2, sub, share.col(i + k % 2)) = f[k];
+      if ((SPAN || (int)sub < used) && share.valid(i + k % 2)) place(k / 2, sub, share.col(i + k % 2)) = f[k];
   }
   __syncthreads();
   if (SPAN) {
@@ -425,7 +427,7 @@ __global__ void __maxnreg__(VALUES == 16 ? 128 : 80) k_norm_backward(NormArgs A,
       float t = 0.f;
       if (c < 2 * A.width) {
 #pragma unroll 8
-        for (int r = part_of; r < (int)rows; r += together) t += place(which, r, c - which * A.width);
+        for (int r = part_of; r < used; r += together) t += place(which, r, c - which * A.width);
       }
       for (int o = together >> 1; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
       if (c < 2 * A.width && part_of == 0) put(which, c - which * A.width, t);
