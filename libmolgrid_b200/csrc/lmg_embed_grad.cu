@@ -145,8 +145,8 @@ __device__ void clear_share(const Clear& C, unsigned block, unsigned blocks) {
   if (block == 0 && threadIdx.x < C.bytes % 16 / 2) reinterpret_cast<unsigned short*>(C.p + C.bytes / 16 * 16)[threadIdx.x] = 0;
 }
 
-// The lanes whose digit of `bits` bits is this lane's, among those with a slot.  By ballots: __match_any_sync took two thirds of the
-// sort's time (25551 slots, 9 bits: 18 us of 30 for the whole gradient).
+// The lanes whose digit of `bits` bits is this lane's, among those with a slot.  A ballot a bit:
+// __match_any_sync took no less, about 1100 cycles a turn of 32 warps.
 __device__ __forceinline__ unsigned same_digit(unsigned digit, int bits, bool slot) {
   unsigned same = __ballot_sync(0xffffffffu, slot);
   for (int b = 0; b < bits; b++) {
@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(SortArgs A) {
 
 // ---- the sort of up to 32768 slots, in one launch -----------------------------------------------------------------------------
 // Eight blocks of a cluster hold an eighth of the slots each, four a thread, and read one another's counts in shared memory; the
-// other clusters of the launch clear the table's gradient meanwhile.  (Two launches a pass: 16384 slots of 50021 types 35 us,
-// 25551 of 350 types 16 us.)
+// other clusters of the launch clear the table's gradient meanwhile.  (Gradients with two launches a
+// pass: 25551 slots of 350 types 30 us instead of 20.7, 16384 of 50021 types and 1024 bfloat16 49 instead of 42.5.)
 constexpr unsigned CLUSTER = 8, CLUSTER_KEYS = 4;
 constexpr int CLUSTER_BITS_MOST = 10;
 

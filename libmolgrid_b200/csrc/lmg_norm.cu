@@ -214,7 +214,8 @@ __device__ __forceinline__ int shift_of(const T* row) { return (int)(reinterpret
 
 // Layer norm with the row in registers: mean, then the squares of what is left.  A block goes from row to row with its weights in
 // registers.  16384 rows of 4096 bfloat16: 104 us with the next row in registers; 91 us with the ring, bound by what it issued with eight
-// values a thread, one at a time and each checked against the row's end; 67 us with sixteen in pairs.
+// values a thread, one at a time and each checked against the row's end; 67 us with sixteen in pairs, 54 with registers for one wave of
+// blocks.
 template <class T, class P, bool SPAN, int VALUES>
 __global__ void __maxnreg__(VALUES == 16 ? 80 : 64) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
                                                              long long out_ld, float* stats) {

@@ -115,25 +115,8 @@ template <int N> struct Bytes;
 template <> struct Bytes<16> { typedef uint4 type; };
 template <> struct Bytes<8> { typedef uint2 type; };
 
-// COLS values of a row from column `col` on, a multiple of COLS, zeros behind its end; VEC: the row begins on 16 bytes, and they are
-// read 16 bytes at a time, or as many as they are
-template <class T, int COLS, bool VEC = true>
-__device__ __forceinline__ void load_cols(const T* row, int col, int width, float (&v)[COLS]) {
-  constexpr int N = !VEC ? COLS : COLS * sizeof(T) < 16 ? COLS : 16 / sizeof(T);
-#pragma unroll
-  for (int k = 0; k < COLS; k += N) {
-    if (VEC && col + k + N <= width) {
-      typename Bytes<VEC ? N * sizeof(T) : 16>::type a = *reinterpret_cast<const typename Bytes<VEC ? N * sizeof(T) : 16>::type*>(row + col + k);
-      const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-      for (int i = 0; i < N; i++) v[k + i] = to_float(e[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; i++) v[k + i] = col + k + i < width ? to_float(row[col + k + i]) : 0.f;
-    }
-  }
-}
-
+// COLS values to a row from column `col` on, a multiple of COLS, those behind its end left out; VEC: the row begins on 16 bytes, and they are
+// written 16 bytes at a time, or as many as they are
 template <class T, int COLS, bool VEC = true>
 __device__ __forceinline__ void store_cols(T* row, int col, int width, const float (&v)[COLS]) {
   constexpr int N = !VEC ? COLS : COLS * sizeof(T) < 16 ? COLS : 16 / sizeof(T);
@@ -153,7 +136,7 @@ __device__ __forceinline__ void store_cols(T* row, int col, int width, const flo
   }
 }
 
-// COLS values of a row as they lie, read long before they are used: half the registers for 16 bits
+// COLS values of a row as they lie, likewise, zeros behind its end: read long before they are used, in half the registers for 16 bits
 template <class T, int COLS, bool VEC = true>
 struct Raw {
   static constexpr int WORDS = COLS * sizeof(T) / 4;
