@@ -47,7 +47,7 @@ template <> __device__ __forceinline__ unsigned packed<__half>(Pair p) {
 template <class T, int VALUES>
 struct Share {
   static constexpr int PER = 16 / sizeof(T), PIECES = VALUES / PER;
-  int thread, n, width, shift;
+  int thread, n, width, shift, before;  // `before`: the values of its first piece that are not the row's yet
   bool full;              // all its values are the row's
   unsigned whole;         // a bit for each piece that is the row's
   unsigned size[PIECES];  // bytes up to the row's end
@@ -55,10 +55,10 @@ struct Share {
 
   static __host__ __device__ __forceinline__ unsigned bytes(unsigned block) { return block * PIECES * 16; }  // of a stage
   __device__ __forceinline__ int col(int i) const { return (thread + n * (i / PER)) * PER + i % PER - shift; }
-  __device__ __forceinline__ bool valid(int i) const { return (unsigned)col(i) < (unsigned)width; }
+  __device__ __forceinline__ bool valid(int i) const { return i % PER * (int)sizeof(T) < (int)size[i / PER] && (i >= PER || i >= before); }
 
   __device__ __forceinline__ Share(int thread_, int n_, int shift_, int width_) : thread(thread_), n(n_), width(width_), shift(shift_) {
-    full = valid(0) && valid(VALUES - 1);
+    before = thread == 0 ? shift : 0;
     whole = 0;
 #pragma unroll
     for (int k = 0; k < PIECES; k++) {
@@ -67,6 +67,7 @@ struct Share {
       off[k] = left > 0 ? n * PER * k : 0;
       whole |= (unsigned)(valid(k * PER) && valid(k * PER + PER - 1)) << k;
     }
+    full = whole == (1u << PIECES) - 1;
   }
   // where its first piece of a row begins
   template <class Q>
@@ -86,7 +87,14 @@ struct Share {
         v[4 * k] = unpack<T>(a.x), v[4 * k + 1] = unpack<T>(a.y), v[4 * k + 2] = unpack<T>(a.z), v[4 * k + 3] = unpack<T>(a.w);
       }
     }
-    cut(v);
+    if (before != 0) {
+#pragma unroll
+      for (int i = 0; i < PER; i += 2) {
+        float f0, f1;
+        split(v[i / 2], f0, f1);
+        v[i / 2] = pair(i < before ? 0.f : f0, i + 1 < before ? 0.f : f1);
+      }
+    }
   }
   __device__ __forceinline__ void store(T* at, const Pair (&v)[VALUES / 2]) const {
 #pragma unroll
@@ -115,10 +123,14 @@ struct Share {
   __device__ __forceinline__ void cut(Pair (&v)[VALUES / 2]) const {
     if (full) return;
 #pragma unroll
-    for (int i = 0; i < VALUES; i += 2) {
-      float f0, f1;
-      split(v[i / 2], f0, f1);
-      v[i / 2] = pair(valid(i) ? f0 : 0.f, valid(i + 1) ? f1 : 0.f);
+    for (int k = 0; k < PIECES; k++) {
+      if (whole >> k & 1) continue;
+#pragma unroll
+      for (int i = k * PER; i < k * PER + PER; i += 2) {
+        float f0, f1;
+        split(v[i / 2], f0, f1);
+        v[i / 2] = pair(valid(i) ? f0 : 0.f, valid(i + 1) ? f1 : 0.f);
+      }
     }
   }
   template <class P>
@@ -215,7 +227,7 @@ __device__ __forceinline__ int shift_of(const T* row) { return (int)(reinterpret
 // Layer norm with the row in registers: mean, then the squares of what is left.  A block goes from row to row with its weights in
 // registers.  16384 rows of 4096 bfloat16: 104 us with the next row in registers; 91 us with the ring, bound by what it issued with eight
 // values a thread, one at a time and each checked against the row's end; 67 us with sixteen in pairs, 54 with registers for one wave of
-// blocks.
+// blocks, 50 with the row's edges seen to only where they are.
 template <class T, class P, bool SPAN, int VALUES>
 __global__ void __maxnreg__(VALUES == 16 ? 80 : 64) k_norm(NormArgs A, const T* x, long long x_ld, const P* weight, const P* bias, T* out,
                                                              long long out_ld, float* stats) {
