@@ -2,9 +2,10 @@
 //
 // Few types, many slots each (k_type_tables): a warp keeps a table of its own in shared memory and adds row after row to
 // it, so the gradients are read once, in order; the blocks' tables are summed afterwards.  Otherwise the slots are sorted by
-// type (a stable radix sort, k_sort_count and k_sort_move), and groups of lanes walk equal pieces of the sorted
-// slots (k_type_pieces): a type that lies within a piece is written at once, one that crosses pieces leaves partial
-// sums that k_type_joins adds up.  Equal pieces, not types, because a type can hold one slot or all of them.  No atomics touch
+// type, and groups of lanes walk equal pieces of the sorted slots: a type that lies within a piece is written at once, one that
+// crosses pieces is put together from partial sums.  In one launch where each block can find its own slots among few
+// (k_type_small) or types are shared out among clusters (k_type_ranges), else by a stable radix sort (k_sort_cluster, or
+// k_sort_count and k_sort_move), k_type_pieces and k_type_joins.  Equal pieces, not types, because a type can hold one slot or all of them.  No atomics touch
 // a sum: its order is fixed by the sizes alone.
 #include "lmg_vectors.h"
 
@@ -262,7 +263,10 @@ struct ClusterSortArgs {
   Clear clear;
 };
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();  // a warp arrives as one
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // what another block of the cluster has at the same place in its shared memory
 __device__ __forceinline__ unsigned cluster_load(const unsigned* p, unsigned rank) {
@@ -434,19 +438,25 @@ struct PieceRow<T, false> {
   __device__ __forceinline__ float get(int c) const { return to_float(v[c]); }
 };
 
-// Sums of a block's sorted slots: keys[1 .. here] and rows[0 .. here - 1], keys[0] and keys[here + 1] those of the slots before and
-// behind.  A group of lanes sums a piece type by type.  A type that crosses pieces is put together in shared memory by the
+// a block's sorted slots: key(1 .. here) and row(0 .. here - 1), key(0) and key(here + 1) those of the slots before and behind
+struct TwoLists {
+  const unsigned *keys, *rows;
+  __device__ __forceinline__ unsigned key(unsigned i) const { return keys[i]; }
+  __device__ __forceinline__ unsigned row(unsigned i) const { return rows[i]; }
+};
+
+// Sums of a block's sorted slots.  A group of lanes sums a piece type by type.  A type that crosses pieces is put together in shared memory by the
 // group that it begins in; only what crosses blocks is left, in `parts` (46 us for 25000 slots, a tenth of them of one type,
 // when every piece left its own).
-template <class T, class O, bool VEC, bool DROP>
-__device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* keys, const unsigned* rows, float* heads, float* tails, unsigned here,
-                                           int col_tile, const T* diff, long long diff_ld, O* grad, long long grad_ld, const Drop& D, float* parts) {
+template <class T, class O, bool VEC, bool DROP, class Sorted>
+__device__ __forceinline__ void sum_pieces(const PieceArgs& A, const Sorted& sorted, float* heads, float* tails, unsigned here, int col_tile,
+                                           const T* diff, long long diff_ld, O* grad, long long grad_ld, const Drop& D, float* parts) {
   constexpr int ROWS = VEC && sizeof(T) == 2 ? 8 : 4;  // whose loads are in flight together
   const int group = threadIdx.x / A.lanes, lane = threadIdx.x % A.lanes;
   const Columns<VEC> C(col_tile, lane, A.lanes, A.width);
   const unsigned begin = min(group * A.piece, here), end = min(begin + A.piece, here);
   const bool some = begin < end && C.any();
-  const unsigned came = keys[begin], goes = keys[end + 1];
+  const unsigned came = sorted.key(begin), goes = sorted.key(end + 1);
   float* head = heads + (size_t)group * A.lanes * 8 + lane * 8;
   float* tail = tails + (size_t)group * A.lanes * 8 + lane * 8;
   auto write = [&](unsigned type, float (&sum)[8]) {
@@ -460,7 +470,7 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
     const int left = A.width - col_tile * A.lanes * 8, first_lane = (threadIdx.x & 31) - lane;
     const unsigned together = (left >= 32 ? ~0u : (1u << min(left, A.lanes)) - 1) >> (left >= 32 ? 32 - A.lanes : 0) << first_lane;
     float sum[8] = {};
-    unsigned type = keys[begin + 1];
+    unsigned type = sorted.key(begin + 1);
     bool first = true;
     auto put = [&](bool last) {
       if (type >= A.ntypes) return;
@@ -478,11 +488,11 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
       PieceRow<T, VEC> v[ROWS];
 #pragma unroll
       for (int j = 0; j < ROWS; j++)
-        if (i + j < end && keys[i + j + 1] < A.ntypes) v[j].load(diff + (long long)rows[i + j] * diff_ld, C);
+        if (i + j < end && sorted.key(i + j + 1) < A.ntypes) v[j].load(diff + (long long)sorted.row(i + j) * diff_ld, C);
 #pragma unroll
       for (int j = 0; j < ROWS; j++) {
         if (i + j >= end) break;
-        const unsigned t = keys[i + j + 1];
+        const unsigned t = sorted.key(i + j + 1);
         if (t != type) {
           put(false);
           first = false;
@@ -492,7 +502,7 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
         }
         if (type >= A.ntypes) continue;
         if (DROP) {
-          const unsigned bits = kept8(D, K, rows[i + j], col_tile * A.lanes + lane);
+          const unsigned bits = kept8(D, K, sorted.row(i + j), col_tile * A.lanes + lane);
 #pragma unroll
           for (int c = 0; c < 8; c++) {
             const int at = lane + c * A.lanes;  // of the tile's columns
@@ -517,7 +527,7 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
 #pragma unroll
       for (int c = 0; c < 8; c++) sum[c] += h[c];
       const unsigned last = min((p + 1) * A.piece, here);
-      if (keys[last] != type || keys[last + 1] != type) return false;
+      if (sorted.key(last) != type || sorted.key(last + 1) != type) return false;
     }
   };
   auto put_part = [&](float* to, const float (&sum)[8]) {
@@ -525,7 +535,7 @@ __device__ __forceinline__ void sum_pieces(const PieceArgs& A, const unsigned* k
     for (int c = 0; c < 8; c++)
       if (C.first + c * C.step < A.width) to[C.first + c * C.step] = sum[c];
   };
-  const unsigned t0 = keys[begin + 1], t1 = keys[end];
+  const unsigned t0 = sorted.key(begin + 1), t1 = sorted.key(end);
   if (group == 0 && t0 == came && t0 < A.ntypes) {
     float sum[8] = {};
     follow(t0, 0, sum);
@@ -552,7 +562,7 @@ __global__ void __launch_bounds__(PIECE_THREADS, DROP ? 2 : 3) k_type_pieces(Pie
     if (i < here) rows[i] = A.row[at];
   }
   __syncthreads();
-  sum_pieces<T, O, VEC, DROP>(A, keys, rows, heads, tails, here, blockIdx.y, diff, diff_ld, grad, grad_ld, D,
+  sum_pieces<T, O, VEC, DROP>(A, TwoLists{keys, rows}, heads, tails, here, blockIdx.y, diff, diff_ld, grad, grad_ld, D,
                                              A.parts + (size_t)blockIdx.x * 2 * A.width);
 }
 
@@ -630,7 +640,139 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_type_small(Slots S, PieceArgs
     }
   if (tid == 0) keys[0] = keys[A.n + 1] = ~0u;
   __syncthreads();
-  sum_pieces<T, O, VEC, DROP>(A, keys, rows, heads, tails, A.n, blockIdx.x, diff, diff_ld, grad, grad_ld, D, nullptr);
+  sum_pieces<T, O, VEC, DROP>(A, TwoLists{keys, rows}, heads, tails, A.n, blockIdx.x, diff, diff_ld, grad, grad_ld, D, nullptr);
+}
+
+// ---- some hundred types, in one launch -------------------------------------------------------------------------------------
+// A cluster has every fifteenth type (types are often numbered by how common they are), a block of it an eighth of the slots: it finds
+// those of its types, in order, sorts them in shared memory, (type, slot) as one word each, and sums them to a table there; the blocks'
+// tables are added up at the end.  (A block alone for a share of the types waits for the one that many slots have: 25551 slots of
+// 350 types, one in eight of one, 37.8 us.)
+constexpr int RANGE_THREADS = 512, RANGE_WARPS = RANGE_THREADS / 32, RANGE_TYPES = 64;
+constexpr unsigned RANGES = 15;  // clusters that fit at once: 16 take 18.9 us for those slots, 15 15.4
+
+__host__ __device__ constexpr unsigned range_share(unsigned rows) {  // slots of a warp
+  return (rows + CLUSTER * RANGE_THREADS - 1) / (CLUSTER * RANGE_THREADS) * 32;
+}
+// shared memory: a block's words, then its lists, a slot and a type for each, whose place the partial sums take in the end, then the table and counts
+__host__ __device__ constexpr size_t range_words(unsigned rows) { return ((size_t)range_share(rows) * RANGE_WARPS + 2 + 3) / 4 * 16; }
+__host__ __device__ constexpr size_t range_lists(unsigned rows) {
+  const size_t lists = (size_t)range_share(rows) * RANGE_WARPS * 3, sums = RANGE_THREADS * 8 * 2 * 4;
+  return lists > sums ? lists : sums;
+}
+size_t range_smem(unsigned rows, unsigned types, int lanes) {
+  return range_words(rows) + range_lists(rows) + (size_t)types * lanes * 32 + RANGE_WARPS * RANGE_TYPES * 4;
+}
+
+struct OneList {
+  const unsigned* words;
+  unsigned first;  // slot of the block
+  __device__ __forceinline__ unsigned key(unsigned i) const { return words[i] >> 16; }
+  __device__ __forceinline__ unsigned row(unsigned i) const { return first + (words[i + 1] & 0xffffu); }
+};
+
+template <class T, class O, bool VEC, bool DROP>
+__global__ void __launch_bounds__(RANGE_THREADS) k_type_ranges(Slots S, PieceArgs A, FastDiv by_ranges, const T* diff, long long diff_ld,
+                                                               O* grad, long long grad_ld, Drop D) {
+  extern __shared__ float4 range_shared[];
+  __shared__ unsigned total;
+  char* shared = reinterpret_cast<char*>(range_shared);
+  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid / 32, lower = (1u << lane) - 1, share = range_share(S.rows);
+  const unsigned rank = blockIdx.x % CLUSTER, range = blockIdx.x / CLUSTER, ranges = by_ranges.d, here_types = (A.ntypes - range + ranges - 1) / ranges;
+  unsigned* words = reinterpret_cast<unsigned*>(shared);
+  unsigned short* slots = reinterpret_cast<unsigned short*>(shared + range_words(S.rows)) + warp * share;
+  unsigned char* types = reinterpret_cast<unsigned char*>(shared + range_words(S.rows)) + 2 * RANGE_WARPS * share + warp * share;
+  float* heads = reinterpret_cast<float*>(shared + range_words(S.rows));
+  float* table = reinterpret_cast<float*>(shared + range_words(S.rows) + range_lists(S.rows));
+  const unsigned cols = A.lanes * 8;
+  unsigned (*count)[RANGE_TYPES] = reinterpret_cast<unsigned (*)[RANGE_TYPES]>(table + here_types * cols);  // of each warp and type
+  for (unsigned i = tid; i < here_types * cols / 4; i += RANGE_THREADS) reinterpret_cast<float4*>(table)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = tid; i < RANGE_WARPS * RANGE_TYPES; i += RANGE_THREADS) count[i / RANGE_TYPES][i % RANGE_TYPES] = 0;
+  __syncthreads();
+  wait_for_stream();
+  const unsigned block_first = rank * share * RANGE_WARPS, begin = block_first + warp * share, end = min(begin + share, S.rows);
+  unsigned found = 0;
+  constexpr int N = 8;  // that are looked up together
+  for (unsigned i0 = begin; i0 < end; i0 += 32 * N) {
+    unsigned row[N];
+    bool in[N];
+    int t[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      row[k] = i0 + k * 32 + lane;
+      in[k] = row[k] < end;
+    }
+    slot_types(S, row, in, t);
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const unsigned type = by_ranges(t[k] < 0 ? 0 : (unsigned)t[k]);
+      const bool mine = t[k] >= 0 && (unsigned)t[k] - type * ranges == range;
+      const unsigned all = __ballot_sync(0xffffffffu, mine);
+      if (mine) {
+        const unsigned at = found + __popc(all & lower);
+        slots[at] = (unsigned short)(row[k] - block_first);
+        types[at] = (unsigned char)type;
+        atomicAdd(&count[warp][type], 1u);
+      }
+      found += __popc(all);
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {  // a lane has two types: where each warp's slots of them go
+    unsigned n[2] = {0, 0};
+#pragma unroll
+    for (int w = 0; w < RANGE_WARPS; w++) {
+      n[0] += count[w][2 * lane];
+      n[1] += count[w][2 * lane + 1];
+    }
+    unsigned run = n[0] + n[1];
+    for (unsigned o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 31) total = run;
+    unsigned at[2] = {run - n[0] - n[1], run - n[1]};
+#pragma unroll
+    for (int w = 0; w < RANGE_WARPS; w++) {
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const unsigned m = count[w][2 * lane + k];
+        count[w][2 * lane + k] = at[k];
+        at[k] += m;
+      }
+    }
+  }
+  __syncthreads();
+  const unsigned here = total;
+  for (unsigned i0 = 0; i0 < found; i0 += 32) {
+    const bool slot = i0 + lane < found;
+    const unsigned type = slot ? types[i0 + lane] : 0, peers = same_digit(type, 6, slot);
+    if (slot) words[1 + count[warp][type] + __popc(peers & lower)] = type << 16 | slots[i0 + lane];
+    __syncwarp();
+    if (slot && (peers & lower) == 0) count[warp][type] += __popc(peers);
+    __syncwarp();
+  }
+  if (tid == 0) words[0] = words[here + 1] = ~0u;
+  __syncthreads();
+  PieceArgs P = A;
+  const unsigned groups = RANGE_THREADS / A.lanes;
+  P.ntypes = here_types;
+  P.piece = max(4u, (here + groups - 1) / groups);  // four slots are one round of loads
+  P.scale = 1.f;
+  sum_pieces<T, float, VEC, DROP>(P, OneList{words, block_first}, heads, heads + RANGE_THREADS * 8, here, 0, diff, diff_ld, table, (long long)cols, D, nullptr);
+  cluster_arrive();
+  cluster_wait();
+  for (unsigned i = rank * RANGE_THREADS + tid; i < here_types * cols; i += CLUSTER * RANGE_THREADS) {
+    const unsigned type = i / cols, col = i % cols;
+    float part[CLUSTER], sum = 0.f;
+#pragma unroll
+    for (unsigned c = 0; c < CLUSTER; c++) part[c] = __uint_as_float(cluster_load(reinterpret_cast<const unsigned*>(table) + i, c));
+#pragma unroll
+    for (unsigned c = 0; c < CLUSTER; c++) sum += part[c];
+    if ((int)col < A.width) grad[(long long)(type * ranges + range) * grad_ld + col] = from_float<O>(sum * A.scale);
+  }
+  cluster_arrive();  // the others read what lies here
+  cluster_wait();
 }
 
 // a type that begins in a block and goes on: its parts, block after block
@@ -672,7 +814,7 @@ __global__ void __launch_bounds__(PIECE_THREADS) k_type_joins(PieceArgs A, O* gr
 
 // ---- the plan: a function of the sizes alone, so that the workspace and the call agree ----------------------------------------
 struct Plan {
-  bool tables, small;
+  bool tables, small, ranges;
   // few types
   unsigned blocks, per;
   int warps;
@@ -690,6 +832,12 @@ constexpr int TABLE_WARPS_LEAST = 4, TABLE_WARPS_MOST = 16;
 // Tiles of 32 columns, and slots times tiles, up to which tables are kept: 200000 slots of 28 types and 128 float32 take 45.5 us with them
 // and 46.5 sorted, of 256 bfloat16 78 and 64, 20000 of 200 float32 10.6 and 23.5.
 constexpr unsigned TABLE_TILES = 8, TABLE_WORK = 1 << 20;
+
+// Slots times columns, and columns, up to which clusters share the types.  In us, shared and sorted: 25551 slots of 350 types and 45 float16
+// 15.4 and 19.7, 10000 of 300 and 8 float32 9 and 33, 60000 of 400 and 128 bfloat16 21 and 27, 20000 of 1900 and 64 float32 17 and 23; 30000 of 300 and
+// 1000 float16 55 and 38, 1500 of 120 and 300 float32 13.2 and 12.5.  Where one type has all slots, which the sizes do not tell, eight blocks
+// do all: the first 51 and 33, without dropout 29 and 31, the third 73 and 55.
+constexpr size_t RANGE_WORK = 1 << 23, RANGE_SMEM = 200 << 10;
 
 Plan plan_for(unsigned rows, int V, int width) {
   Plan p = {};
@@ -731,6 +879,19 @@ Plan plan_for(unsigned rows, int V, int width) {
     p.blocks = (V + p.per - 1) / p.per;
     p.bytes = 256;
     return p;
+  }
+  if (V <= (int)(2 * RANGES * RANGE_TYPES) && width <= 256 && (size_t)rows * width <= RANGE_WORK) {
+    p.lanes = 1;
+    while (p.lanes < 32 && p.lanes * 8 < width) p.lanes *= 2;
+    unsigned ranges = ((unsigned)V + RANGE_TYPES - 1) / RANGE_TYPES;
+    if (ranges < RANGES) ranges = RANGES;
+    p.per = (V + ranges - 1) / ranges;
+    p.blocks = ranges < (unsigned)V ? ranges : V;
+    if (range_smem(rows, p.per, p.lanes) <= RANGE_SMEM) {
+      p.ranges = true;
+      p.bytes = 256;
+      return p;
+    }
   }
   int key_bits = 1, most = 1;
   while (key_bits < 31 && (unsigned)V >> key_bits) key_bits++;
@@ -808,6 +969,26 @@ cudaError_t by_network(const Slots& S, const Plan& p, const lmg_vectors* diff, c
   ++*launches;
   return launch_early(kernel, dim3(sums + p.blocks), SMALL_THREADS, 0, st, S, P, sums, p.per, FastDiv(vec ? (unsigned)(width + 7) / 8 : (unsigned)width),
                       static_cast<const T*>(diff->data), diff->ld, static_cast<O*>(grad->data), grad->ld, D);
+}
+
+template <class T, class O>
+cudaError_t by_ranges(const Slots& S, const Plan& p, const lmg_vectors* diff, const lmg_vectors* grad, int width, float scale, const Drop& D,
+                      char*, long* launches, cudaStream_t st) {
+  PieceArgs P = {};
+  P.n = S.rows;
+  P.ntypes = (unsigned)S.ntypes;
+  P.lanes = p.lanes;
+  P.width = width;
+  P.scale = scale;
+  const bool vec = rows_aligned(diff);
+  const auto kernel = vec ? (drops(D) ? k_type_ranges<T, O, true, true> : k_type_ranges<T, O, true, false>)
+                          : (drops(D) ? k_type_ranges<T, O, false, true> : k_type_ranges<T, O, false, false>);
+  const size_t smem = range_smem(S.rows, p.per, p.lanes);
+  const cudaError_t e = allow_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
+  ++*launches;
+  return launch_clusters(kernel, p.blocks * CLUSTER, CLUSTER, RANGE_THREADS, smem, st, S, P, FastDiv(p.blocks), static_cast<const T*>(diff->data),
+                         diff->ld, static_cast<O*>(grad->data), grad->ld, D);
 }
 
 template <class T, class O>
@@ -919,7 +1100,8 @@ int lmg_embed_types_backward(const lmg_slots* slots, int ntypes, int width, cons
   const Drop D = to_drop(drop);
   long launches = 0;
   const cudaError_t e = by_vector_types<false, true>(diff->type, table_gradients->type, [&](auto t, auto o) {
-    const auto by = p.tables ? by_tables<decltype(t), decltype(o)> : p.small ? by_network<decltype(t), decltype(o)> : by_sort<decltype(t), decltype(o)>;
+    const auto by = p.tables ? by_tables<decltype(t), decltype(o)> : p.small ? by_network<decltype(t), decltype(o)>
+                    : p.ranges ? by_ranges<decltype(t), decltype(o)> : by_sort<decltype(t), decltype(o)>;
     return by(S, p, diff, table_gradients, width, scale, D, static_cast<char*>(workspace), &launches, st);
   });
   lmg_internal_count_launches(launches);

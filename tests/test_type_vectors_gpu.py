@@ -97,6 +97,11 @@ LOOKUPS = [
     ((3000,), 30, 300, F, F, F, 0.0, 0, 0), ((700,), 20, 1000, B, B, F, 0.3, 0, 0), ((1025,), 4000, 20, F, F, torch.int32, 0.0, 0, 0),
     ((1024,), 4000, 21, F, F, torch.int32, 0.4, 0, 0), ((1024,), 2097151, 4, F, F, torch.int32, 0.0, 0, 0),
     ((900,), 2097152, 4, F, F, torch.int32, 0.0, 0, 0), ((32768,), 113, 16, F, F, torch.int32, 0.0, 0, 0),
+    # types shared out among clusters: 64 of a cluster, twice as many clusters as fit at once, and one type too many; widths and lengths at the ends
+    ((5000,), 960, 8, F, F, torch.int32, 0.0, 0, 0), ((4097,), 961, 17, F, F, F, 0.2, 0, 1), ((5000,), 1920, 9, H, H, torch.int64, 0.0, 0, 0),
+    ((5000,), 1921, 9, H, H, torch.int64, 0.0, 0, 0), ((1100,), 113, 1, H, H, F, 0.5, 0, 0), ((20000,), 960, 256, B, B, F, 0.2, 0, 0),
+    ((1500,), 121, 256, F, B, F, 0.0, 8, 0), ((100000,), 200, 83, F, F, torch.int32, 0.0, 0, 0), ((7, 25001), 350, 40, F, H, F, 0.1, 0, 0),
+    ((300000,), 350, 20, F, F, F, 0.0, 0, 0),
 ]
 IDS = ["%s-%dx%d-%s" % ("x".join(map(str, c[0])), c[1], c[2], str(c[4])[6:]) for c in LOOKUPS]
 
