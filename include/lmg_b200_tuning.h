@@ -26,6 +26,10 @@ unsigned lmg_tma_timeouts(void);
  * fill}; collecting synchronises the recorded events. */
 int lmg_profile_enable(int max_records);
 int lmg_profile_collect(double ms[3], int count[3]);
+/* How a layer norm of `rows` rows is laid out, rows >= 1, 1 <= width < 2^30; slack: how many values the 16 bytes that a row begins in may
+ * have before it (0 where all rows begin on 16 bytes, else 3 of float32 and 7 of 16 bits).  plan = {1 for the kernels of wide rows; rows that a
+ * block has at once; how many times as many rows there are; blocks of lmg_layer_norm; blocks of lmg_layer_norm_backward}.  Nothing is launched. */
+void lmg_norm_plan(int rows, int width, int slack, unsigned plan[5]);
 /* Kernels this library has launched in this process. */
 long lmg_launch_count(void);
 

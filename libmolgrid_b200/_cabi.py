@@ -132,6 +132,7 @@ EXTRA_SYMBOLS = [
     # bench support
     ("lmg_profile_enable", ctypes.c_int, [ctypes.c_int]),
     ("lmg_profile_collect", ctypes.c_int, [ctypes.POINTER(ctypes.c_double), c_int_p]),
+    ("lmg_norm_plan", None, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_uint)]),
     ("lmg_launch_count", ctypes.c_long, []),
 ]
 

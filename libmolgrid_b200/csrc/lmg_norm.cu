@@ -569,6 +569,7 @@ __global__ void __launch_bounds__(256) k_norm_weights_wide(NormArgs A, unsigned 
 struct NormPlan {
   bool wide;
   int values, threads, block;       // a thread's values of a row; threads of a row, of a block
+  unsigned rows;                    // that a block has at once
   unsigned tiles, forward, blocks;  // blocks of the two passes
   unsigned per;                     // rows of a block of the wide sums
   size_t bytes;
@@ -588,6 +589,7 @@ NormPlan norm_plan(unsigned rows, int width, int slack) {
     if (p.threads * p.values < most) p.threads = (most + p.values * 32 - 1) / (p.values * 32) * 32;
     p.block = p.threads > 32 ? p.threads : BLOCK;
     const unsigned per = p.threads > 32 ? 1 : BLOCK / p.threads;
+    p.rows = per;
     p.tiles = (rows + per - 1) / per;
     // blocks an SM holds: by the stages of float32, whatever the type, so that sums go by the sizes alone, and by registers.  148 and its
     // multiples by a block's rows, or by 2: as many rows apart as it takes for a thread's rows to begin alike in their 16 bytes
@@ -603,8 +605,9 @@ NormPlan norm_plan(unsigned rows, int width, int slack) {
     // four rows a block and more, so that the sums are no more than the rows; one block needs no other launch for them (2.8 us)
     if (per == 1 && p.blocks > 148 && p.blocks > p.tiles / 4) p.blocks = p.tiles / 4 > 148 ? p.tiles / 4 / 8 * 8 : 148;
     if (p.blocks > p.tiles) p.blocks = p.tiles;
-    if (per == 1 && slack && p.blocks < p.tiles) p.blocks = p.blocks < 8 ? 1 : p.blocks / 8 * 8;
-    if (p.tiles <= 4) p.blocks = 1;
+    const bool any = per > 1 || slack == 0;  // number of blocks lets a thread's rows begin alike
+    if (!any && p.blocks < p.tiles) p.blocks = p.blocks / 8 * 8;
+    if (any && p.tiles <= 4) p.blocks = 1;
   }
   p.bytes = 256 + (size_t)p.blocks * 2 * width * 4;
   return p;
@@ -620,6 +623,12 @@ bool alike(const lmg_vectors* a, const lmg_vectors* b) {
 NormPlan plan_of(unsigned rows, int width, const lmg_vectors* x, bool all_alike) {
   if (!all_alike) return norm_plan(rows, width, WIDE);
   return norm_plan(rows, width, rows_aligned(x) ? 0 : 16 / (int)element_bytes(x->type) - 1);
+}
+
+// Threads keep the place in 16 bytes at which their first row begins: a pass whose threads have more than one has to jump by whole ones.
+int check_jump(const NormPlan& p, unsigned blocks, const lmg_vectors* x) {
+  if (p.wide || blocks >= p.tiles || (unsigned long long)p.rows * blocks * x->ld * element_bytes(x->type) % 16 == 0) return LMG_OK;
+  return vectors_fail(LMG_ERR_INVALID_ARGUMENT, "rows of a thread begin at different places in their 16 bytes");
 }
 
 // dynamic shared memory of a pass over `arrays` arrays
@@ -663,6 +672,15 @@ size_t lmg_vectors_workspace_bytes(int op, int rows, int ntypes, int width) {
   return most;
 }
 
+void lmg_norm_plan(int rows, int width, int slack, unsigned plan[5]) {
+  const lmg::NormPlan p = lmg::norm_plan((unsigned)rows, width, slack);
+  plan[0] = p.wide;
+  plan[1] = p.rows;
+  plan[2] = p.tiles;
+  plan[3] = p.forward;
+  plan[4] = p.blocks;
+}
+
 int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const void* weight, const void* bias, int weight_type,
                    float eps, const lmg_vectors* out, float* stats, void* stream) {
   using namespace lmg;
@@ -675,6 +693,7 @@ int lmg_layer_norm(const lmg_slots* rows, int width, const lmg_vectors* x, const
   if ((rc = check_weights(x->type, weight_type)) || (rc = check_stats(stats))) return rc;
   NormArgs A = {to_slots(rows, 0), width, 0, 0, eps};
   const NormPlan p = plan_of(A.S.rows, width, x, alike(x, out));
+  if ((rc = check_jump(p, p.forward, x))) return rc;
   A.threads = p.threads;
   A.tiles = p.tiles;
   const cudaError_t e = by_types(x->type, weight_type, [&](auto t, auto q) {
@@ -717,6 +736,7 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
   }
   NormArgs A = {to_slots(rows, 0), width, 0, 0, 0.f};
   const NormPlan p = none ? norm_plan(0, width, 0) : plan_of(A.S.rows, width, x, alike(x, diff) && alike(x, x_gradients));
+  if (!none && (rc = check_jump(p, p.blocks, x))) return rc;
   A.threads = p.threads;
   A.tiles = p.tiles;
   if (workspace == nullptr || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
