@@ -357,8 +357,8 @@ enum { LMG_OP_EMBED_BACKWARD = 16, LMG_OP_LAYER_NORM_BACKWARD = 17 };
  * fail with LMG_ERR_WORKSPACE on a smaller one, and on one that does not start on 16 bytes. */
 size_t lmg_vectors_workspace_bytes(int op, int rows, int ntypes, int width);
 
-/* Reads back (synchronising `stream`) the status word that kernels of the last call that used
- * `workspace` wrote: 0, or LMG_ERR_OUT_OF_RANGE / LMG_ERR_INVALID_ARGUMENT when an atom's type
+/* Reads back (synchronising `stream`) the status word that kernels of the last gridding call that used
+ * `workspace` wrote (0 where one of the gradients above has written to it since): 0, or LMG_ERR_OUT_OF_RANGE / LMG_ERR_INVALID_ARGUMENT when an atom's type
  * index was >= ntypes - the data-dependent checks of src/grid_maker.cpp:172 and :458-460,
  * which the reference makes on the host while it loops over atoms. */
 int lmg_check_status(void* workspace, void* stream);

@@ -213,10 +213,12 @@ class _Workspaces(threading.local):
 
 
 _workspaces = _Workspaces()
+# of what is no gridding call: what GridMaker.check_types reads stays where the last gridding call left it
+_other_workspaces = _Workspaces()
 _transform_ring = {}   # (device, batch) -> pinned staging buffers of GridMaker.batch_transforms
 
 
-def _workspace(device, nbytes, least=None):
+def _workspace(device, nbytes, least=None, kept=_workspaces):
     """Scratch buffer of the current stream, reused across calls (grown on demand).  Given up, it goes back to
     torch's allocator for that stream, whose order keeps it from calls still under way.  A call that is being captured has
     one of its own, in the memory of its graph.  Where there is no room for ``nbytes``, one of ``least``."""
@@ -230,7 +232,7 @@ def _workspace(device, nbytes, least=None):
 
     if torch.cuda.is_current_stream_capturing():
         return room()
-    by, key = _workspaces.by, torch._C._cuda_getCurrentRawStream(device.index) << 6 | device.index
+    by, key = kept.by, torch._C._cuda_getCurrentRawStream(device.index) << 6 | device.index
     ws = by.pop(key, None)
     if ws is None or ws.numel() < nbytes:
         if len(by) >= _Workspaces.KEPT:

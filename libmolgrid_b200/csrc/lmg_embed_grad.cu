@@ -25,6 +25,7 @@ __global__ void __launch_bounds__(512) k_type_tables(Slots S, unsigned per, cons
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, warps = blockDim.x / 32, V = S.ntypes, q = lane / TABLE_LANES, l = lane % TABLE_LANES;
   for (int i = threadIdx.x; i < warps * 4 * V * TABLE_LANES; i += blockDim.x) tables[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   wait_for_stream();
+  if (gridDim.x > 1) no_status(parts);
   const DropKey K(D);
   float4* mine = tables + (size_t)(warp * 4 + q) * V * TABLE_LANES + l;
   const int col = blockIdx.y * TABLE_COLS + l * 4;
@@ -161,6 +162,7 @@ __device__ __forceinline__ unsigned same_digit(unsigned digit, int bits, bool sl
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_count(SortArgs A) {
   __shared__ unsigned count[1 << SORT_BITS_MOST];
   wait_for_stream();
+  if (A.key_in == nullptr) no_status(A.key_out);
   if (blockIdx.x >= A.tiles) return clear_share(A.clear, blockIdx.x - A.tiles, gridDim.x - A.tiles);
   const unsigned bins = 1u << A.bits;
   for (unsigned b = threadIdx.x; b < bins; b += SORT_THREADS) count[b] = 0;
@@ -280,6 +282,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A
   extern __shared__ unsigned sort_shared[];
   __shared__ unsigned warp_sum[SORT_WARPS];
   wait_for_stream();
+  no_status(A.key[0]);
   if (blockIdx.x >= CLUSTER) return clear_share(A.clear, blockIdx.x - CLUSTER, gridDim.x - CLUSTER);
   const unsigned bins = 1u << A.bits, mask = bins - 1, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, block = blockIdx.x;
   unsigned* count = sort_shared;                                            // [bins] of this block
@@ -850,7 +853,7 @@ constexpr size_t RANGE_WORK = 1 << 23, RANGE_SMEM = 200 << 10;
 Plan plan_for(unsigned rows, int V, int width) {
   Plan p = {};
   if (V == 0 || width == 0 || rows == 0) {
-    p.bytes = 256;
+    p.bytes = STATUS_FRONT;
     return p;
   }
   // tables: four a warp; fewer than four warps an SM have too few loads in flight
@@ -868,7 +871,7 @@ Plan plan_for(unsigned rows, int V, int width) {
       const unsigned warps = p.blocks * p.warps;
       p.per = ((rows + warps - 1) / warps + 31) / 32 * 32;
       p.blocks = (unsigned)(((unsigned long long)rows + (unsigned long long)p.per * p.warps - 1) / ((unsigned long long)p.per * p.warps));
-      p.bytes = 256 + (size_t)p.blocks * V * width * 4;
+      p.bytes = STATUS_FRONT + (size_t)p.blocks * V * width * 4;
       return p;
     }
   }
@@ -885,7 +888,7 @@ Plan plan_for(unsigned rows, int V, int width) {
     if (blocks < ((unsigned)V + SMALL_RANGE - 1) / SMALL_RANGE) blocks = ((unsigned)V + SMALL_RANGE - 1) / SMALL_RANGE;
     p.per = (V + blocks - 1) / blocks;  // types of a block
     p.blocks = (V + p.per - 1) / p.per;
-    p.bytes = 256;
+    p.bytes = STATUS_FRONT;
     return p;
   }
   if (V <= (int)(2 * RANGES * RANGE_TYPES) && width <= 256 && (size_t)rows * width <= RANGE_WORK) {
@@ -897,7 +900,7 @@ Plan plan_for(unsigned rows, int V, int width) {
     p.blocks = ranges < (unsigned)V ? ranges : V;
     if (range_smem(rows, p.per, p.lanes) <= RANGE_SMEM) {
       p.ranges = true;
-      p.bytes = 256;
+      p.bytes = STATUS_FRONT;
       return p;
     }
   }
@@ -925,7 +928,7 @@ Plan plan_for(unsigned rows, int V, int width) {
   while (p.piece < 32 && p.piece < want && p.piece * 2 * (PIECE_THREADS / p.lanes) <= PIECE_SLOTS) p.piece *= 2;
   const unsigned slots = p.piece * (PIECE_THREADS / p.lanes);
   p.piece_blocks = (rows + slots - 1) / slots;
-  size_t at = 256;
+  size_t at = STATUS_FRONT;
   for (int k = 0; k < 2; k++) {
     p.key[k] = at;
     at += aligned256((size_t)rows * 4);
@@ -943,7 +946,7 @@ Plan plan_for(unsigned rows, int V, int width) {
 template <class T, class O>
 cudaError_t by_tables(const Slots& S, const Plan& p, const lmg_vectors* diff, const lmg_vectors* grad, int width, float scale, const Drop& D,
                       char* ws, long* launches, cudaStream_t st) {
-  float* parts = reinterpret_cast<float*>(ws + 256);
+  float* parts = reinterpret_cast<float*>(ws + STATUS_FRONT);
   O* g = static_cast<O*>(grad->data);
   const bool vec = rows_aligned(diff);
   const auto kernel = vec ? (drops(D) ? k_type_tables<T, O, true, true> : k_type_tables<T, O, true, false>)

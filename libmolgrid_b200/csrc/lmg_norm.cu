@@ -326,6 +326,7 @@ __global__ void __maxnreg__(VALUES == 16 ? 128 : 80) k_norm_backward(NormArgs A,
   const unsigned array = share.bytes(blockDim.x), stage = 2 * array + blockDim.x * 8, ring_at = (unsigned)__cvta_generic_to_shared(ring);
   RowSum<SPAN, 2> sum(part, n);
   wait_for_stream();
+  if (SUMS && gridDim.x > 1) no_status(parts);
   const T *x_from = share.first(x + (long long)row * x_ld), *g_from = share.first(diff + (long long)row * diff_ld);
   T* to = share.first(grad + (long long)row * grad_ld);
   const unsigned jump = rows * gridDim.x;
@@ -544,6 +545,7 @@ __global__ void __launch_bounds__(256) k_norm_weights_wide(NormArgs A, unsigned 
                                                            long long diff_ld, float* parts) {
   __shared__ float s[2][8][32];
   wait_for_stream();
+  no_status(parts);
   const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, slice = threadIdx.x / 32;
   const unsigned begin = blockIdx.y * per, end = min(begin + per, A.S.rows);
   float dw = 0.f, db = 0.f;
@@ -609,7 +611,7 @@ NormPlan norm_plan(unsigned rows, int width, int slack) {
     if (!any && p.blocks < p.tiles) p.blocks = p.blocks / 8 * 8;
     if (any && p.tiles <= 4) p.blocks = 1;
   }
-  p.bytes = 256 + (size_t)p.blocks * 2 * width * 4;
+  p.bytes = STATUS_FRONT + (size_t)p.blocks * 2 * width * 4;
   return p;
 }
 
@@ -749,7 +751,7 @@ int lmg_layer_norm_backward(const lmg_slots* rows, int width, const lmg_vectors*
     return e == cudaSuccess ? LMG_OK : vectors_cuda(e, "gradients of a layer norm");
   }
   const bool sums = weight_gradients || bias_gradients;
-  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + STATUS_FRONT);
   long launches = 0;
   const cudaError_t e = by_types(x->type, weight_type, [&](auto t, auto q) {
     typedef decltype(t) T;

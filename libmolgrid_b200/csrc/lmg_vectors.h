@@ -28,6 +28,8 @@ struct FastDiv {
 #endif
 };
 
+constexpr size_t STATUS_FRONT = 256;  // bytes of a workspace before the scratch of these calls
+
 struct Slots {
   unsigned rows, n;  // batch * max_atoms, max_atoms
   FastDiv by_n;
@@ -101,6 +103,12 @@ __device__ __forceinline__ int slot_type(const Slots& S, unsigned row) {
   int t[1];
   slot_types(S, rows, in, t);
   return t[0] < 0 ? -1 : t[0];
+}
+
+// The front of a workspace is what lmg_check_status() reads: it goes with flags behind it, so the first launch of a call that writes there takes
+// it away.
+__device__ __forceinline__ void no_status(void* scratch) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *reinterpret_cast<unsigned long long*>(static_cast<char*>(scratch) - STATUS_FRONT) = 0;
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }

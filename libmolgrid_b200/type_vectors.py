@@ -21,7 +21,7 @@ from . import _cabi
 from . import api as _api
 from . import grids as _grids
 from ._cabi import check
-from .api import _Arg, _current_device, _fast, _stream_ptr, _workspace, _workspaces
+from .api import _Arg, _current_device, _fast, _other_workspaces, _stream_ptr, _workspace
 
 _VECTORS = {torch.float32: _cabi.FLOAT32, torch.bfloat16: _cabi.BFLOAT16, torch.float16: _cabi.FLOAT16}
 _INDICES = {torch.float32: _cabi.INDEX_FLOAT32, torch.int32: _cabi.INDEX_INT32, torch.int64: _cabi.INDEX_INT64}
@@ -203,7 +203,7 @@ def embed_types_backward(types, diff, table_gradients, scale=1.0, n_atoms=None, 
     vectors; types without a slot get zero.  16-bit gradients may go into a float32 table."""
     m = _api._native or _fast()
     if m and m._fast_embed_backward(types, diff, table_gradients, scale, n_atoms, p, rng,
-            status, _workspaces.by) is not None:
+            status, _other_workspaces.by) is not None:
         return
     dev = _current_device()
     t, s, keep = _types(types, n_atoms, dev, status)
@@ -213,7 +213,7 @@ def embed_types_backward(types, diff, table_gradients, scale=1.0, n_atoms=None, 
     V, W = int(g.t.shape[0]), int(g.t.shape[1])
     d = _Vectors(diff, dev, "diff").shaped(tuple(t.shape) + (W,), "diff")
     drop = _drop(p, rng, dev)
-    ws = _workspace(dev, _cabi.lib().lmg_vectors_workspace_bytes(_cabi.OP_EMBED_BACKWARD, s.batch * s.max_atoms, V, W))
+    ws = _workspace(dev, _cabi.lib().lmg_vectors_workspace_bytes(_cabi.OP_EMBED_BACKWARD, s.batch * s.max_atoms, V, W), kept=_other_workspaces)
     check(_cabi.lib().lmg_embed_types_backward(ctypes.byref(s), V, W, ctypes.byref(d.struct), float(scale), _ref(drop),
                                                ctypes.byref(g.struct), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
                                                _stream_ptr(dev)))
@@ -267,7 +267,7 @@ def layer_norm_backward(x, weight, stats, diff, x_gradients, weight_gradients=No
     be ``diff``; gradients of weights or biases that are not wanted are None."""
     m = _api._native or _fast()
     if m and m._fast_layer_norm_backward(x, weight, stats, diff, x_gradients, weight_gradients,
-            bias_gradients, n_atoms, _workspaces.by) is not None:
+            bias_gradients, n_atoms, _other_workspaces.by) is not None:
         return
     dev = _current_device()
     a = _Vectors(x, dev, "x")
@@ -280,7 +280,8 @@ def layer_norm_backward(x, weight, stats, diff, x_gradients, weight_gradients=No
     st = _dense(stats, dev, "stats", {torch.float32: 0}, tuple(a.t.shape[:-1]) + (2,))
     s, keep = _slots(a.t.shape[:-1], n_atoms, dev)
     W = int(a.t.shape[-1])
-    ws = _workspace(dev, _cabi.lib().lmg_vectors_workspace_bytes(_cabi.OP_LAYER_NORM_BACKWARD, s.batch * s.max_atoms, 0, W))
+    ws = _workspace(dev, _cabi.lib().lmg_vectors_workspace_bytes(_cabi.OP_LAYER_NORM_BACKWARD, s.batch * s.max_atoms, 0, W),
+                    kept=_other_workspaces)
     check(_cabi.lib().lmg_layer_norm_backward(ctypes.byref(s), W, ctypes.byref(a.struct), _data(w), wtype, _data(st),
                                               ctypes.byref(d.struct), ctypes.byref(g.struct), _data(dw), _data(db),
                                               ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(dev)))

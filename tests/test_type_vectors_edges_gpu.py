@@ -51,3 +51,89 @@ def test_norm_modules_of_few_wide_rows():
     m = lmg.TypeVectors(3, 1001, device="cuda", seed=5)
     m(torch.tensor([0, 2, 1, 2], device="cuda")).backward(normal(g, 4, 1001))
     assert all(bool(torch.isfinite(v.grad).all()) for v in m.parameters())
+
+
+# ---- what GridMaker.check_types reads ---------------------------------------------------------------------------------
+GRADIENTS = [
+    # slots, types, width: few types, many types (one cluster sorts; several launches)
+    ("tables", lambda: table_gradient(20000, 28, 28)), ("sort", lambda: table_gradient(20000, 5000, 64)),
+    ("long sort", lambda: table_gradient(40000, 5000, 24)), ("norm", lambda: norm_gradient(3000, 28)), ("wide norm", lambda: norm_gradient(200, 8200)),
+    ("small", lambda: table_gradient(500, 5000, 24)),
+]
+
+
+def table_gradient(n, V, W):
+    g = gen(5)
+    types = torch.randint(0, V, (n,), generator=g, device="cuda", dtype=torch.int32)
+    lmg.embed_types_backward(types, normal(g, n, W), torch.empty(V, W, device="cuda"))
+
+
+def norm_gradient(n, W):
+    g = gen(5)
+    x = normal(g, n, W)
+    out, stats, dw = torch.empty_like(x), torch.empty(n, 2, device="cuda"), torch.empty(W, device="cuda")
+    lmg.layer_norm(x, None, None, out, stats)
+    lmg.layer_norm_backward(x, None, stats, out, torch.empty_like(x), dw, torch.empty_like(dw))
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["compiled", "general"])
+@pytest.mark.parametrize("gradient", [c[1] for c in GRADIENTS], ids=[c[0] for c in GRADIENTS])
+def test_gradients_leave_what_check_types_reads(gradient, native, monkeypatch):
+    from libmolgrid_b200 import api
+    if not native:
+        monkeypatch.setattr(api, "_native", False)
+    g = gen(1)
+    gm = lmg.GridMaker(0.5, 7.5)
+    n, C = 3000, 4
+    coords, radii = (torch.rand(n, 3, generator=g, device="cuda") - 0.5) * 6, torch.ones(n, device="cuda")
+    grid = torch.empty(gm.grid_dimensions(C), device="cuda")
+    good = torch.randint(0, C, (n,), generator=g, device="cuda").float()
+    bad = good.clone()
+    bad[1234] = C
+    for _ in range(2):     # the second time with buffers that there are already
+        gm.forward((0, 0, 0), coords, good, radii, grid)
+        gradient()
+        gm.check_types()
+        gm.forward((0, 0, 0), coords, bad, radii, grid)
+        gradient()
+        with pytest.raises(IndexError):
+            gm.check_types()
+
+
+def test_training_step_leaves_what_check_types_reads():
+    g = gen(3)
+    B, N, V, C = 4, 2000, 28, 6
+    gm = lmg.GridMaker(0.5, 7.5)
+    m = lmg.TypeVectors(V, C, seed=3, device="cuda")
+    c2g = lmg.Coords2Grid(gm, types=m)
+    coords, radii = (torch.rand(B, N, 3, generator=g, device="cuda") - 0.5) * 6, torch.ones(B, N, device="cuda")
+    types = torch.randint(0, V, (B, N), generator=g, device="cuda").float()
+    for _ in range(2):
+        out = c2g(coords, types, radii)
+        out.backward(normal(g, *out.shape))
+        gm.check_types()
+        m.check_types()
+
+
+@pytest.mark.parametrize("n,V,W", [(20000, 28, 28), (20000, 5000, 64), (40000, 5000, 24)])
+def test_a_workspace_that_a_gradient_took_has_no_status(n, V, W):
+    """At the C interface one workspace may serve both: what a gradient wrote over is not read as a gridding call's flags."""
+    import ctypes
+    from libmolgrid_b200 import _cabi, api
+    lib = _cabi.lib()
+    g = gen(7)
+    gm = lmg.GridMaker(0.5, 7.5)
+    types = torch.randint(0, V, (n,), generator=g, device="cuda").float()
+    coords, radii = (torch.rand(n, 3, generator=g, device="cuda") - 0.5) * 6, torch.ones(n, device="cuda")
+    gm.forward((0, 0, 0), coords, types, radii, torch.empty(gm.grid_dimensions(4), device="cuda"))   # types beyond the channels
+    ws, st = gm._last_ws, api._stream_ptr(torch.device("cuda", torch.cuda.current_device()))
+    assert lib.lmg_check_status(ctypes.c_void_p(ws.data_ptr()), st) == _cabi.LMG_ERR_OUT_OF_RANGE
+    big = torch.empty(lib.lmg_vectors_workspace_bytes(_cabi.OP_EMBED_BACKWARD, n, V, W) + ws.numel(), dtype=torch.uint8, device="cuda")
+    big[:ws.numel()] = ws
+    s = _cabi.SlotsStruct()
+    s.batch, s.max_atoms, s.type_index, s.index_type = 1, n, types.data_ptr(), _cabi.INDEX_FLOAT32
+    diff, grad = normal(g, n, W), torch.empty(V, W, device="cuda")
+    vec = [_cabi.VectorsStruct(t.data_ptr(), _cabi.FLOAT32, W) for t in (diff, grad)]
+    _cabi.check(lib.lmg_embed_types_backward(ctypes.byref(s), V, W, ctypes.byref(vec[0]), 1.0, None, ctypes.byref(vec[1]),
+                                             ctypes.c_void_p(big.data_ptr()), big.numel(), st))
+    assert lib.lmg_check_status(ctypes.c_void_p(big.data_ptr()), st) == _cabi.LMG_OK
