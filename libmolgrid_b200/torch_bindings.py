@@ -78,7 +78,8 @@ class Coords2Grid(torch.nn.Module):
     """Module form: ``Coords2Grid(gmaker, center=(0,0,0))(coords, types, radii)``.
 
     ``types=`` takes a module that makes type vectors of type indices, such as ``TypeVectors(ntypes, channels)``: ``types``
-    may then be indices (N,) or (B,N), with ``n_atoms`` (B,) in padded batches, and gradients reach the module's table."""
+    may then be indices (N,) or (B,N), with ``n_atoms`` (B,) in padded batches, and gradients reach the module's table.  A
+    ``draw`` is handed to that module."""
 
     def __init__(self, gmaker, center=(0, 0, 0), types=None):
         super().__init__()
@@ -86,11 +87,11 @@ class Coords2Grid(torch.nn.Module):
         self.center = center
         self.types = types
 
-    def forward(self, coords, types, radii, n_atoms=None):
+    def forward(self, coords, types, radii, n_atoms=None, draw=None):
         if self.types is not None and types.dim() == coords.dim() - 1:
-            types = self.types(types) if n_atoms is None else self.types(types, n_atoms)
-        elif n_atoms is not None:
-            raise ValueError("n_atoms goes with type indices that a module turns into vectors")
+            types = self.types(types, *(() if n_atoms is None else (n_atoms,)), **({} if draw is None else {"draw": draw}))
+        elif n_atoms is not None or draw is not None:
+            raise ValueError("n_atoms and draw go with type indices that a module turns into vectors")
         coords, types, radii = coords.contiguous(), types.contiguous(), radii.contiguous()
         single = coords.dim() == 2 and types.dim() == 2 and radii.dim() == 1
         batched = coords.dim() == 3 and types.dim() == 3 and radii.dim() == 2

@@ -435,21 +435,32 @@ class _Drawing(torch.nn.Module):
         seed = int(torch.randint(1 << 62, (1,)).item()) if seed is None else int(seed)
         self.register_buffer("generator", generator_state(seed, device or "cpu"))
 
-    def _draw(self):
+    def draw(self):
+        """One draw of the module's generator, to be given to a call - or to the two of a pass that is computed again in the
+        backward pass (``torch.utils.checkpoint``); None where nothing is dropped."""
+        return next_draw(self.generator) if self.training and self.p > 0.0 else None
+
+    def _draw(self, given):
         """(p, draw) of this call."""
         if not self.training or self.p == 0.0:
             return 0.0, None
-        return self.p, next_draw(self.generator)
+        if given is None:
+            if torch._C._current_graph_task_id() != -1:   # a backward pass is under way
+                raise RuntimeError("a pass that is computed again would drop other values than the first time: give both the same "
+                                   "draw, forward(..., draw=module.draw())")
+            given = next_draw(self.generator)
+        return self.p, given
 
 
 class Dropout(_Drawing):
-    """Dropout of the last dimension's values while training, without a stored mask."""
+    """Dropout of the last dimension's values while training, without a stored mask.  ``draw`` as :func:`dropout` takes it
+    (:meth:`draw`, or a seed and an offset); without it each call takes the generator's next."""
 
     def __init__(self, p=0.5, seed=None, device=None):
         super().__init__(p, seed, device)
 
-    def forward(self, x):
-        p, draw = self._draw()
+    def forward(self, x, draw=None):
+        p, draw = self._draw(draw)
         return x if draw is None else DropoutFunction.apply(x, p, draw)
 
     def extra_repr(self):
@@ -480,7 +491,7 @@ class TypeVectors(_Drawing):
     ``TypeVectors(ntypes, width)(types[, n_atoms])`` with ``types`` (N,) or (B,N), or a ``DeviceBatch``.  Every slot of a type
     has the same normalised row, so the table is normalised, not the slots, and the gradients of all slots of a type are
     summed before they go through the norm.  The scale goes into the norm's eps there: layer_norm(s x, eps) is layer_norm(x, eps / s^2).
-    A type >= ntypes is an empty slot; :meth:`check_types` raises for it."""
+    A type >= ntypes is an empty slot; :meth:`check_types` raises for it.  ``draw`` as in :class:`Dropout`."""
 
     def __init__(self, ntypes, width, scale=1.0, norm=True, p=0.0, eps=1e-5, seed=None, dtype=torch.float32, device=None):
         super().__init__(p, seed, device)
@@ -498,13 +509,13 @@ class TypeVectors(_Drawing):
             self.register_parameter("bias", None)
         self.register_buffer("status", torch.zeros(1, dtype=torch.int32, device=device), persistent=False)
 
-    def forward(self, types, n_atoms=None):
+    def forward(self, types, n_atoms=None, draw=None):
         from .coord_cache import DeviceBatch
         if isinstance(types, DeviceBatch):
             if n_atoms is not None:
                 raise TypeError("a DeviceBatch has atom counts of its own")
             types, n_atoms = types.type_index, types.n_atoms
-        p, draw = self._draw()
+        p, draw = self._draw(draw)
         table, scale = self.table, self.scale
         if self.weight is not None:
             table, scale = LayerNormFunction.apply(table, self.weight, self.bias, self.eps / scale ** 2, None), 1.0

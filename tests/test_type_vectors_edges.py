@@ -32,3 +32,11 @@ def test_workspace_covers_every_alignment(lib, slack):
         for n in (1, 2, 3, 4, 5, 100, 1000, 20000):
             lib.lmg_norm_plan(n, width, slack, plan)
             assert lib.lmg_vectors_workspace_bytes(_cabi.OP_LAYER_NORM_BACKWARD, n, 0, width) >= 256 + plan[4] * 2 * width * 4
+
+
+def test_draws_go_with_type_indices():
+    import torch
+    import libmolgrid_b200 as lmg
+    with pytest.raises(ValueError):
+        lmg.Coords2Grid(lmg.GridMaker(0.5, 5.5))(torch.zeros(2, 4, 3), torch.zeros(2, 4, 2), torch.ones(2, 4), draw=(1, 0))
+    assert lmg.Dropout(0.0).draw() is None and lmg.TypeVectors(3, 2, p=0.5).eval().draw() is None

@@ -137,3 +137,72 @@ def test_a_workspace_that_a_gradient_took_has_no_status(n, V, W):
     _cabi.check(lib.lmg_embed_types_backward(ctypes.byref(s), V, W, ctypes.byref(vec[0]), 1.0, None, ctypes.byref(vec[1]),
                                              ctypes.c_void_p(big.data_ptr()), big.numel(), st))
     assert lib.lmg_check_status(ctypes.c_void_p(big.data_ptr()), st) == _cabi.LMG_OK
+
+
+# ---- passes that are computed again -----------------------------------------------------------------------------------
+def gradients(m, call, up):
+    for v in m.parameters():
+        v.grad = None
+    out = call()
+    out.backward(up)
+    return [out.detach()] + [v.grad.clone() for v in m.parameters()]
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_a_checkpointed_module_has_the_same_gradients(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    g = gen(8)
+    V, W, n = 20, 16, 500
+    types = torch.randint(0, V, (n,), generator=g, device="cuda")
+    m = torch.nn.Sequential(lmg.TypeVectors(V, W, p=0.3, seed=3, device="cuda"), lmg.Dropout(0.4, seed=4, device="cuda"))
+    vectors, drop = m
+    up, leaf = normal(g, n, W), torch.zeros((), device="cuda", requires_grad=True)   # a reentrant pass wants an input with a gradient
+    a, b = vectors.draw(), drop.draw()
+    assert a.tolist() == [3, 0] and vectors.generator.tolist() == [3, 1]
+
+    def forward(z):
+        return drop(vectors(types, draw=a), draw=b) + z
+    want = gradients(m, lambda: forward(leaf), up)
+    got = gradients(m, lambda: checkpoint(forward, leaf, use_reentrant=reentrant), up)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    assert vectors.generator.tolist() == [3, 1] and drop.generator.tolist() == [4, 1]
+    # without a draw the pass would take others the second time
+    for again in (lambda z: vectors(types) + z, lambda z: drop(vectors(types, draw=a)) + z):
+        out = checkpoint(again, leaf, use_reentrant=reentrant)
+        with pytest.raises(RuntimeError, match="draw"):
+            out.backward(up)
+    m.eval()
+    want = gradients(m, lambda: drop(vectors(types)) + leaf, up)
+    got = gradients(m, lambda: checkpoint(lambda z: drop(vectors(types)) + z, leaf, use_reentrant=reentrant), up)
+    assert all(torch.equal(p, q) for p, q in zip(want, got)) and vectors.draw() is None
+
+
+def test_a_given_draw():
+    m = lmg.Dropout(0.5, seed=9, device="cuda")
+    x = torch.ones(40, 24, device="cuda")
+    first = m(x)                                             # draw 0 of its own
+    assert torch.equal(m(x, draw=(9, 0)), first) and m.generator.tolist() == [9, 1]
+    assert torch.equal(m(x, draw=torch.tensor([9, 0], device="cuda")), first)
+    assert torch.equal(m.eval()(x, draw=(9, 0)), x)
+    with pytest.raises(ValueError):
+        m.train()(x, draw=(9, 1 << 63))
+
+
+def test_types_to_grids_computed_again():
+    from torch.utils.checkpoint import checkpoint
+    g = gen(10)
+    B, N, V, C = 2, 30, 9, 5
+    gm = lmg.GridMaker(0.5, 7.5)
+    m = lmg.TypeVectors(V, C, p=0.4, seed=3, device="cuda")
+    c2g = lmg.Coords2Grid(gm, types=m)
+    coords = ((torch.rand(B, N, 3, generator=g, device="cuda") - 0.5) * 6).requires_grad_()
+    radii, types = torch.ones(B, N, device="cuda"), torch.randint(0, V, (B, N), generator=g, device="cuda").float()
+    na, draw = torch.tensor([30, 11], dtype=torch.int32, device="cuda"), m.draw()
+    up = normal(g, B, *gm.grid_dimensions(C))
+    want = gradients(m, lambda: c2g(coords, types, radii, na, draw=draw), up)
+    got = gradients(m, lambda: checkpoint(lambda c: c2g(c, types, radii, na, draw=draw), coords, use_reentrant=False), up)
+    # densities and gradients of atoms are summed in an order that varies; the table's are not
+    for p, q in zip(want, got):
+        torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-5)
+    with pytest.raises(ValueError):
+        lmg.Coords2Grid(gm)(coords, torch.zeros(B, N, C, device="cuda"), radii, draw=draw)
