@@ -424,8 +424,11 @@ class DropoutFunction(torch.autograd.Function):
 # modules
 # ------------------------------------------------------------------------------------------------
 class _Drawing(torch.nn.Module):
-    """A module that drops values in training.  Its generator is a buffer: it moves with the module to the GPU and with
-    the state dict from run to run.  Without ``seed`` torch's host generator gives one."""
+    """A module that drops values in training.  Its generator moves with the module to the GPU and with the state dict from run to
+    run.  Without ``seed`` torch's host generator gives one.  It is a rank's own and no buffer, which ``DistributedDataParallel`` would
+    copy from rank 0: ranks that are to drop different values get different seeds."""
+
+    _ranks_own = ("generator",)   # tensors that move with the module
 
     def __init__(self, p, seed, device):
         super().__init__()
@@ -433,7 +436,33 @@ class _Drawing(torch.nn.Module):
         if not 0.0 <= self.p <= 1.0:
             raise ValueError("dropout probability outside [0, 1]")
         seed = int(torch.randint(1 << 62, (1,)).item()) if seed is None else int(seed)
-        self.register_buffer("generator", generator_state(seed, device or "cpu"))
+        self.generator = generator_state(seed, device or "cpu")
+
+    def _apply(self, fn, *args, **kw):
+        super()._apply(fn, *args, **kw)
+        for name in self._ranks_own:
+            setattr(self, name, fn(getattr(self, name)))
+        return self
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "generator"] = self.generator
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        key = prefix + "generator"
+        if key in unexpected_keys:
+            unexpected_keys.remove(key)
+        given = state_dict.get(key)
+        if given is None:
+            if strict:
+                missing_keys.append(key)
+        elif not torch.is_tensor(given) or given.dtype is not torch.int64 or tuple(given.shape) != (2,):
+            error_msgs.append("%s: expected the seed and the offset of a generator, two int64" % key)
+        elif local_metadata.get("assign_to_params_buffers"):
+            self.generator = given
+        else:
+            self.generator.copy_(given)
 
     def draw(self):
         """One draw of the module's generator, to be given to a call - or to the two of a pass that is computed again in the
@@ -493,6 +522,8 @@ class TypeVectors(_Drawing):
     summed before they go through the norm.  The scale goes into the norm's eps there: layer_norm(s x, eps) is layer_norm(x, eps / s^2).
     A type >= ntypes is an empty slot; :meth:`check_types` raises for it.  ``draw`` as in :class:`Dropout`."""
 
+    _ranks_own = ("generator", "status")
+
     def __init__(self, ntypes, width, scale=1.0, norm=True, p=0.0, eps=1e-5, seed=None, dtype=torch.float32, device=None):
         super().__init__(p, seed, device)
         self.scale, self.eps, self.dtype = float(scale), float(eps), dtype
@@ -507,7 +538,7 @@ class TypeVectors(_Drawing):
         else:
             self.register_parameter("weight", None)
             self.register_parameter("bias", None)
-        self.register_buffer("status", torch.zeros(1, dtype=torch.int32, device=device), persistent=False)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
 
     def forward(self, types, n_atoms=None, draw=None):
         from .coord_cache import DeviceBatch
