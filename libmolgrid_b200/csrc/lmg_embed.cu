@@ -299,8 +299,9 @@ cudaError_t launch_rows(const Slots& S, const lmg_vectors* src, const lmg_vector
   const bool aligned = rows_aligned(src) && rows_aligned(out);
   const bool flat = out->ld == width && reinterpret_cast<uintptr_t>(out->data) % 16 == 0 &&
                     (LOOKUP || (src->ld == width && reinterpret_cast<uintptr_t>(src->data) % 16 == 0));
-  // passes of less than 2^30 values, a multiple of eight rows so that each begins on 16 bytes again
-  const unsigned most = width > 1 << 26 ? 0 : (1u << 30) / (unsigned)width & ~7u;
+  // passes of less than 2^30 values, a multiple of eight rows so that each begins on 16 bytes again; wider rows would be more than the 65535
+  // tiles of 256 groups of four columns that a launch has
+  const unsigned most = width > 65535 * 1024 ? 0 : (1u << 30) / (unsigned)width & ~7u;
   return by_vector_types<LOOKUP, false>(src->type, out->type, [&](auto t, auto o) {
     typedef decltype(t) T;
     typedef decltype(o) O;

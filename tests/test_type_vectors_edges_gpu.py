@@ -206,3 +206,19 @@ def test_types_to_grids_computed_again():
         torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-5)
     with pytest.raises(ValueError):
         lmg.Coords2Grid(gm)(coords, torch.zeros(B, N, C, device="cuda"), radii, draw=draw)
+
+
+# ---- the widest rows --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("W", [65535 * 1024, 65535 * 1024 + 4, 65535 * 1024 + 1, 1 << 26, (1 << 26) + 4])
+def test_the_widest_rows(W):
+    table = torch.arange(W, device="cuda", dtype=F)[None]
+    out = torch.full((2, W), 5.0, device="cuda")
+    lmg.embed_types(torch.tensor([0, -1], device="cuda"), table, out, 2.0)
+    assert torch.equal(out[0], table[0] * 2) and not out[1].any()
+    lmg.dropout(out, out, 0.0, (1, 0))
+    assert torch.equal(out[0], table[0] * 2)
+    lmg.dropout(table, out[:1], 0.5, (1, 0))
+    kept = torch.from_numpy(plain.draws(1, 4096, (1, 0)) >= 2.0 ** 31).cuda()
+    assert torch.equal(out[0, 1:4096] != 0, kept[0, 1:])
+    stays = out[0] != 0
+    assert torch.equal(out[0][stays], table[0][stays] * 2) and abs(float(stays.double().mean()) - 0.5) < 5 * 0.5 / W ** 0.5
