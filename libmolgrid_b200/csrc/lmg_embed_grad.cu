@@ -904,7 +904,7 @@ Plan plan_for(unsigned rows, int V, int width) {
       return p;
     }
   }
-  int key_bits = 1, most = 1;
+  int key_bits = 2, most = 2;  // two bits a pass at least, with more than 2^30 slots too: 31 bits take 16 passes
   while (key_bits < 31 && (unsigned)V >> key_bits) key_bits++;
   if (rows <= CLUSTER * CLUSTER_KEYS * SORT_THREADS) {
     p.tile = (rows + CLUSTER * SORT_THREADS - 1) / (CLUSTER * SORT_THREADS) * SORT_THREADS;
@@ -918,7 +918,6 @@ Plan plan_for(unsigned rows, int V, int width) {
   }
   p.passes = (key_bits + most - 1) / most;
   p.bits = (key_bits + p.passes - 1) / p.passes;
-  if (p.bits < 2) p.bits = 2;
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes * 8 < width) p.lanes *= 2;
   const unsigned cols = (width + p.lanes * 8 - 1) / (p.lanes * 8);

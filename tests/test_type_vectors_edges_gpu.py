@@ -222,3 +222,22 @@ def test_the_widest_rows(W):
     assert torch.equal(out[0, 1:4096] != 0, kept[0, 1:])
     stays = out[0] != 0
     assert torch.equal(out[0][stays], table[0][stays] * 2) and abs(float(stays.double().mean()) - 0.5) < 5 * 0.5 / W ** 0.5
+
+
+# ---- more slots than 2^30 ---------------------------------------------------------------------------------------------
+def test_gradient_of_more_than_a_billion_slots():
+    from libmolgrid_b200 import _cabi, api
+    R, V = (1 << 30) + 5, 100000      # 17 bits of keys, two a pass: nine passes of two launches, the sums and what crosses their blocks
+    types = torch.arange(R, device="cuda", dtype=torch.int32).remainder_(V)
+    diff = types.remainder(7).add_(1).to(B)[:, None]
+    grad = torch.full((V, 1), 5.0, device="cuda")
+    n = _cabi.lib().lmg_launch_count()
+    lmg.embed_types_backward(types, diff, grad)
+    launches = _cabi.lib().lmg_launch_count() - n
+    t = torch.arange(V, device="cuda")
+    slots = R // V + (t < R % V)
+    assert torch.equal(grad[:, 0].double(), slots.double() * (t % 7 + 1))     # whole numbers below 2^24: exact in any order
+    assert launches == 20
+    api._other_workspaces.clear()
+    del types, diff
+    torch.cuda.empty_cache()
