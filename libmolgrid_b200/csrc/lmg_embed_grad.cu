@@ -266,10 +266,13 @@ struct ClusterSortArgs {
 };
 
 __device__ __forceinline__ void cluster_arrive() {
-  __syncwarp();  // a warp arrives as one
+  __syncwarp();  // a warp arrives as one, and waits as one
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // what another block of the cluster has at the same place in its shared memory
 __device__ __forceinline__ unsigned cluster_load(const unsigned* p, unsigned rank) {
   unsigned v;
