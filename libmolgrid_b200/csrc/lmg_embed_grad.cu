@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_move(SortArgs A) {
 // pass: 25551 slots of 350 types 30 us instead of 20.7, 16384 of 50021 types and 1024 bfloat16 49 instead of 42.5.)
 constexpr unsigned CLUSTER = 8, CLUSTER_KEYS = 4;
 constexpr int CLUSTER_BITS_MOST = 10;
+static_assert(1 << CLUSTER_BITS_MOST <= SORT_THREADS, "a thread has one digit");
 
 struct ClusterSortArgs {
   Slots S;
@@ -338,21 +339,20 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A
     }
     cluster_arrive();
     cluster_wait();
-    // digits' totals to their first places; a thread has two digits at most
-    unsigned sum[2] = {0, 0}, off[2] = {0, 0};
-    const unsigned b0 = bins > SORT_THREADS ? 2 * tid : tid, nb = bins > SORT_THREADS ? 2 : b0 < bins ? 1 : 0;
-    for (unsigned k = 0; k < nb; k++) {
+    // digits' totals to their first places, a digit a thread
+    unsigned sum = 0, off = 0;
+    if (tid < bins) {
 #pragma unroll
       for (unsigned c = 0; c < CLUSTER; c++) {
-        const unsigned n = cluster_load(count + b0 + k, c);
-        sum[k] += n;
-        off[k] += c < block ? n : 0;
+        const unsigned n = cluster_load(count + tid, c);
+        sum += n;
+        off += c < block ? n : 0;
       }
     }
     const bool last = pass == A.passes - 1;
     __syncthreads();
     if (last) cluster_arrive();  // the others' counts have been read: they may leave once all have come here
-    unsigned run = sum[0] + sum[1];
+    unsigned run = sum;
     for (unsigned o = 1; o < 32; o <<= 1) {
       const unsigned up = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += up;
@@ -361,9 +361,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_cluster(ClusterSortArgs A
     __syncthreads();
     unsigned before = lane < warp ? warp_sum[lane] : 0;
     before = __reduce_add_sync(0xffffffffu, before);
-    const unsigned first = run - sum[0] - sum[1] + before;
-    if (nb > 0) base[b0] = first + off[0];
-    if (nb > 1) base[b0 + 1] = first + sum[0] + off[1];
+    if (tid < bins) base[tid] = run - sum + before + off;
     __syncthreads();
     unsigned *key_out = A.key[pass & 1], *row_out = A.row[pass & 1];
 #pragma unroll
