@@ -529,6 +529,9 @@ class TypeVectors(_Drawing):
         self.scale, self.eps, self.dtype = float(scale), float(eps), dtype
         if norm and not self.scale > 0.0:
             raise ValueError("scale must be positive where its result is normalised")
+        float32 = torch.finfo(torch.float32)
+        if norm and not float32.tiny <= self._norm_eps() <= float32.max:
+            raise ValueError("eps / scale^2, the norm's eps on the table itself, is beyond float32")
         if dtype not in _VECTORS:
             raise ValueError("dtype: %s is none of %s" % (dtype, ", ".join(str(d) for d in _VECTORS)))
         self.table = torch.nn.Parameter(torch.randn(int(ntypes), int(width), device=device))
@@ -540,6 +543,10 @@ class TypeVectors(_Drawing):
             self.register_parameter("bias", None)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
 
+    def _norm_eps(self):
+        square = self.scale * self.scale
+        return self.eps / square if square > 0.0 else float("inf")
+
     def forward(self, types, n_atoms=None, draw=None):
         from .coord_cache import DeviceBatch
         if isinstance(types, DeviceBatch):
@@ -549,7 +556,7 @@ class TypeVectors(_Drawing):
         p, draw = self._draw(draw)
         table, scale = self.table, self.scale
         if self.weight is not None:
-            table, scale = LayerNormFunction.apply(table, self.weight, self.bias, self.eps / scale ** 2, None), 1.0
+            table, scale = LayerNormFunction.apply(table, self.weight, self.bias, self._norm_eps(), None), 1.0
         return EmbedTypesFunction.apply(types, table, self.dtype, scale, n_atoms, p, draw, self.status)
 
     def check_types(self):

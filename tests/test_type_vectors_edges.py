@@ -110,3 +110,16 @@ def test_generators_in_state_dicts():
         twin.load_state_dict(dict(state, **{"1.generator": torch.zeros(3)}))
     m = m.half().to("meta")
     assert m[0].generator.dtype is torch.int64 and m[0].generator.is_meta and m[0].status.is_meta and m[0].table.dtype is torch.float16
+
+
+@pytest.mark.parametrize("bad", [dict(scale=1e20), dict(scale=1e-25), dict(scale=1e200), dict(scale=1e-200), dict(scale=float("nan")), dict(scale=float("inf")),
+                                 dict(eps=0.0), dict(eps=-1e-5), dict(eps=1e-44), dict(eps=float("nan"))])
+def test_scales_that_take_eps_out_of_range(bad):
+    """The norm of scale * row is that of the row with eps / scale^2, which float32 has to hold."""
+    import libmolgrid_b200 as lmg
+    with pytest.raises(ValueError):
+        lmg.TypeVectors(3, 2, **bad)
+    lmg.TypeVectors(3, 2, scale=1e16)
+    lmg.TypeVectors(3, 2, scale=1e-21)
+    if "scale" in bad:
+        lmg.TypeVectors(3, 2, norm=False, **bad)
