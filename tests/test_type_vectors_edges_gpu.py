@@ -241,3 +241,89 @@ def test_gradient_of_more_than_a_billion_slots():
     api._other_workspaces.clear()
     del types, diff
     torch.cuda.empty_cache()
+
+
+# ---- padded batches to grids ------------------------------------------------------------------------------------------
+class Shifted(torch.nn.Module):
+    """Vectors with something added to all of them, empty slots too."""
+
+    def __init__(self, V, C):
+        super().__init__()
+        self.vectors, self.shift = lmg.TypeVectors(V, C, seed=1, device="cuda"), torch.nn.Parameter(torch.full((C,), 0.7, device="cuda"))
+
+    def forward(self, types, n_atoms=None):
+        return self.vectors(types, n_atoms) + self.shift
+
+
+@pytest.mark.parametrize("maker", ["python", "compiled"])
+@pytest.mark.parametrize("counts", ["list", "int32", "int64"])
+def test_padding_is_not_gridded(maker, counts):
+    if maker == "python":
+        gm = lmg.GridMaker(0.5, 7.5)
+    else:
+        import molgrid
+        gm = molgrid.GridMaker(0.5, 7.5)
+    g = gen(16)
+    B, N, V, C = 4, 40, 9, 6
+    na = [40, 0, 13, 1]
+    coords = (torch.rand(B, N, 3, generator=g, device="cuda") - 0.5) * 6
+    radii = torch.rand(B, N, generator=g, device="cuda") + 1.0
+    types = torch.randint(0, V, (B, N), generator=g, device="cuda").float()
+    m = Shifted(V, C)
+    up = normal(g, B, *gm.grid_dimensions(C))
+    want = []
+    for b, n in enumerate(na):
+        c = coords[b, :n].clone().requires_grad_()
+        out = lmg.Coords2Grid(gm, types=m)(c, types[b, :n], radii[b, :n])
+        out.backward(up[b])
+        want.append((out.detach(), c.grad))
+    shift = m.shift.grad.clone()
+    for fill in (None, float("nan"), 1e30, float("inf")):
+        if fill is not None:
+            for b, n in enumerate(na):
+                coords[b, n:], radii[b, n:], types[b, n:] = fill, fill, fill
+        for v in m.parameters():
+            v.grad = None
+        c = coords.clone().requires_grad_()
+        counted = na if counts == "list" else torch.tensor(na, dtype=getattr(torch, counts), device="cuda")
+        out = lmg.Coords2Grid(gm, types=m)(c, types, radii, counted)
+        out.backward(up)
+        for b, n in enumerate(na):
+            # sums of up to 40 densities and of some thousand voxels, whose order goes by the batch
+            torch.testing.assert_close(out[b], want[b][0], rtol=1e-5, atol=1e-5)
+            torch.testing.assert_close(c.grad[b, :n], want[b][1], rtol=1e-4, atol=1e-3)
+            assert not c.grad[b, n:].any()
+        torch.testing.assert_close(m.shift.grad, shift, rtol=1e-4, atol=1e-2)
+
+
+def test_padding_and_second_derivatives():
+    g = gen(17)
+    B, N, V, C = 3, 20, 9, 4
+    gm = lmg.GridMaker(0.5, 7.5)
+    na = [20, 0, 7]
+    coords = (torch.rand(B, N, 3, generator=g, device="cuda") - 0.5) * 6
+    radii, types = torch.ones(B, N, device="cuda"), torch.randint(0, V, (B, N), generator=g, device="cuda").float()
+    m = Shifted(V, C)
+    up, v = normal(g, B, *gm.grid_dimensions(C)), normal(g, B, N, 3)
+
+    def forces(b, n, c, counted):
+        out = lmg.Coords2Grid(gm, types=m)(c, types if counted else types[b, :n], radii if counted else radii[b, :n],
+                                           *([counted] if counted else []))
+        up_ = (up if counted else up[b]).clone().requires_grad_()
+        f, = torch.autograd.grad(out, c, up_, create_graph=True)
+        return torch.autograd.grad(f, [up_, m.shift], v if counted else v[b, :n], retain_graph=False)
+
+    one = [forces(b, n, coords[b, :n].clone().requires_grad_(), None) for b, n in enumerate(na) if n]
+    for b, n in enumerate(na):
+        coords[b, n:], radii[b, n:] = float("nan"), float("nan")
+    all_up, all_shift = forces(0, 0, coords.clone().requires_grad_(), na)
+    for (u, _), b in zip(one, (0, 2)):
+        torch.testing.assert_close(all_up[b], u, rtol=1e-4, atol=1e-3)
+    assert not all_up[1].any()
+    torch.testing.assert_close(all_shift, one[0][1] + one[1][1], rtol=1e-4, atol=1e-2)
+
+
+def test_counts_without_a_batch():
+    gm, m = lmg.GridMaker(0.5, 7.5), Shifted(3, 4)
+    with pytest.raises(ValueError):
+        lmg.Coords2Grid(gm, types=m)(torch.zeros(5, 3, device="cuda"), torch.zeros(5, device="cuda"), torch.ones(5, device="cuda"), [5])
