@@ -327,3 +327,162 @@ def test_counts_without_a_batch():
     gm, m = lmg.GridMaker(0.5, 7.5), Shifted(3, 4)
     with pytest.raises(ValueError):
         lmg.Coords2Grid(gm, types=m)(torch.zeros(5, 3, device="cuda"), torch.zeros(5, device="cuda"), torch.ones(5, device="cuda"), [5])
+
+
+# ---- the ends of the ranges of a table --------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,V,W,p", [(5, 3, 1 << 20, 0.3), (5, 3, (1 << 20) + 8, 0.3), (7, 2, 1 << 23, 0.0), (1100, 40, 70001, 0.2)])
+def test_gradients_of_wide_tables(rows, V, W, p):
+    g = gen(W)
+    types = torch.randint(-1, V, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    diff = normal(g, rows, W, dtype=H)
+    grad, check = guarded((V, W), F)
+    lmg.embed_types_backward(types, diff, grad, 0.5, p=p, rng=(3, 4))
+    plain.assert_near(grad, *plain.embed_backward(types, diff, V, 0.5, None, p, (3, 4)))
+    check()
+
+
+def test_the_most_types():
+    """2^31 - 1 rows of one value: keys of 31 bits, and addresses beyond them."""
+    V = (1 << 31) - 1
+    table = torch.zeros(V, 1, dtype=B, device="cuda")
+    some = torch.tensor([0, 1, V - 1, 1 << 30, V - 2, 12345678], device="cuda")
+    table[some, 0] = torch.arange(1, 7, device="cuda").to(B)
+    types = some.repeat(500)
+    types[7] = V                                   # beyond the table
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.empty(types.shape[0], 1, dtype=B, device="cuda")
+    lmg.embed_types(types, table, out, status=status)
+    want = torch.arange(1, 7, device="cuda").repeat(500)
+    want[7] = 0
+    assert torch.equal(out[:, 0].long(), want) and int(status) == 1
+    table.fill_(3.0)
+    lmg.embed_types_backward(types, torch.ones_like(out), table)
+    assert table[some, 0].tolist() == [500] * 6    # 499 of the second: halfway between 498 and 500, whose last bit of eight is even
+    table[some] = 0
+    assert not bool(table.view(torch.int16).any())
+    for kind in (torch.int32, F):                  # what float32 holds: 2^31 - 1 is no number of it
+        few = torch.tensor([1 << 30, 5, -1], device="cuda").to(kind)
+        lmg.embed_types_backward(few.repeat(600), torch.ones(1800, 1, dtype=B, device="cuda"), table)
+        assert table[[1 << 30, 5, 0], 0].tolist() == [600, 600, 0]
+        table[[1 << 30, 5]] = 0
+        assert not bool(table.view(torch.int16).any())
+    del table
+    torch.cuda.empty_cache()
+
+
+def test_gradients_into_rows_with_gaps_beyond_4_gb():
+    g = gen(23)
+    V, W, rows = 70000, 32768, 1100
+    grad, check = guarded((V, W), B, 8)
+    types = torch.randint(0, V, (rows,), generator=g, device="cuda")
+    types[-40:] = torch.tensor([V - 1, 3], device="cuda").repeat(20)
+    diff = normal(g, rows, W, dtype=B)
+    grad.fill_(9.0)
+    lmg.embed_types_backward(types, diff, grad)
+    check()
+    met = types.unique()
+    rank = torch.searchsorted(met, types)
+    want, tol = plain.embed_backward(rank, diff, met.numel(), 1.0, None, 0.0, None)
+    plain.assert_near(grad[met], want, tol)
+    grad[met] = 0
+    assert not bool(grad.view(V, W).any())
+    del grad, check
+    torch.cuda.empty_cache()
+
+
+def test_rows_with_gaps_captured():
+    """A table's gradient that is cleared before the sort, in a graph."""
+    g = gen(24)
+    V, W, rows = 5000, 24, 9000
+    types, diff = torch.randint(0, V, (rows,), generator=g, device="cuda"), normal(g, rows, W)
+    grad, check = guarded((V, W), F, 4)
+    lmg.embed_types_backward(types, diff, grad)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lmg.embed_types_backward(types, diff, grad)
+    for seed in (25, 26):
+        types.copy_(torch.randint(0, V, (rows,), generator=gen(seed), device="cuda"))
+        grad.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        plain.assert_near(grad, *plain.embed_backward(types, diff, V, 1.0, None, 0.0, None))
+        check()
+
+
+# ---- batches assembled on the GPU -------------------------------------------------------------------------------------
+def test_types_of_a_device_batch(tmp_path):
+    import numpy as np
+    from libmolgrid_b200 import coord_cache
+    rng = np.random.default_rng(3)
+    lines = []
+    for i in range(4):
+        for name, n in (("r%d.gninatypes" % i, int(rng.integers(20, 90))), ("l%d.gninatypes" % i, int(rng.integers(3, 30)))):
+            coord_cache.write_gninatypes(tmp_path / name, rng.normal(size=(n, 3)) * 3, rng.integers(0, 30, n))
+        lines.append("1 0.5 r%d.gninatypes l%d.gninatypes" % (i, i))
+    (tmp_path / "list.types").write_text("\n".join(lines) + "\n")
+    p = coord_cache.ExampleProvider(data_root=str(tmp_path))
+    p.populate(str(tmp_path / "list.types"))
+    batch = p.next_device_batch(4)
+    batch.check()
+    V, W = batch.num_types(), 6
+    types, na = batch.type_index, batch.n_atoms
+    g = gen(4)
+    table = normal(g, V, W)
+    out, again = (torch.full(tuple(types.shape) + (W,), 5.0, device="cuda") for _ in range(2))
+    lmg.embed_types(batch, table, out)
+    lmg.embed_types(types, table, again, n_atoms=na)
+    assert torch.equal(out, again)
+    plain.assert_near(out, *plain.embed(types, table, 1.0, na, 0.0, None))
+    up, grad, want = normal(g, *out.shape), torch.empty_like(table), torch.empty_like(table)
+    lmg.embed_types_backward(batch, up, grad)
+    lmg.embed_types_backward(types, up, want, n_atoms=na)
+    assert torch.equal(grad, want)
+    m = lmg.TypeVectors(V, W, device="cuda", seed=1)
+    assert torch.equal(m(batch), m(types, na))
+    for call in (lambda: lmg.embed_types(batch, table, out, n_atoms=na), lambda: m(batch, na)):
+        with pytest.raises(TypeError):
+            call()
+    c2g = lmg.Coords2Grid(lmg.GridMaker(0.5, 7.5), types=m)
+    grids = c2g(batch.coords, types, batch.radii, na)
+    grids.sum().backward()
+    assert bool(torch.isfinite(grids).all()) and all(bool(torch.isfinite(v.grad).all()) for v in m.parameters())
+    m.check_types()
+
+
+# ---- threads ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("own_streams", [True, False])
+def test_threads_at_once(own_streams):
+    """Calls of four threads, whose scratch differs in size and lies under way together."""
+    import threading
+    g = gen(30)
+    inputs, want = [], []
+    for k, (n, V, W) in enumerate([(20000, 28, 28), (20000, 5000, 64), (40000, 5000, 24), (9000, 60, 300)]):
+        types, x = torch.randint(0, V, (n,), generator=g, device="cuda"), normal(g, n, W)
+        inputs.append((types, x, V))
+
+    def step(types, x, V):
+        grad, out, stats = torch.empty(V, x.shape[1], device="cuda"), torch.empty_like(x), torch.empty(x.shape[0], 2, device="cuda")
+        dw, dx = torch.empty(x.shape[1], device="cuda"), torch.empty_like(x)
+        lmg.embed_types_backward(types, x, grad)
+        lmg.layer_norm(x, None, None, out, stats)
+        lmg.layer_norm_backward(x, None, stats, out, dx, dw)
+        return grad, out, dx, dw
+    want = [step(*i) for i in inputs]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(k):
+        stream = torch.cuda.Stream() if own_streams else torch.cuda.current_stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = step(*inputs[k])
+                stream.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, want[k])):
+                    failures.append(k)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
