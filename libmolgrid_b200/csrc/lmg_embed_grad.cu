@@ -842,7 +842,8 @@ struct Plan {
 constexpr size_t TABLE_SMEM = SMEM_MOST;  // an SM's
 constexpr int TABLE_WARPS_LEAST = 4, TABLE_WARPS_MOST = 16;
 // Tiles of 32 columns, and slots times tiles, up to which tables are kept: 200000 slots of 28 types and 128 float32 take 45.5 us with them
-// and 46.5 sorted, of 256 bfloat16 78 and 64, 20000 of 200 float32 10.6 and 23.5.
+// and 46.5 sorted, of 256 bfloat16 78 and 64, 20000 of 200 float32 10.6 and 23.5.  Set by four tiles: of one tile (28 columns) tables take 36.8 for
+// 1048576 slots, and one slot more, sorted, 73.
 constexpr unsigned TABLE_TILES = 8, TABLE_WORK = 1 << 20;
 
 // Slots times columns, and columns, up to which clusters share the types.  In us, shared and sorted: 25551 slots of 350 types and 45 float16
