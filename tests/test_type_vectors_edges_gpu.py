@@ -296,18 +296,21 @@ def test_padding_is_not_gridded(maker, counts):
         torch.testing.assert_close(m.shift.grad, shift, rtol=1e-4, atol=1e-2)
 
 
-def test_padding_and_second_derivatives():
+@pytest.mark.parametrize("by_type", [False, True], ids=["radii by atom", "radii by type"])
+@pytest.mark.parametrize("maker", ["python", "compiled"])
+def test_padding_and_second_derivatives(maker, by_type):
+    import molgrid
     g = gen(17)
     B, N, V, C = 3, 20, 9, 4
-    gm = lmg.GridMaker(0.5, 7.5)
+    gm = (lmg if maker == "python" else molgrid).GridMaker(0.5, 7.5, False, by_type)
     na = [20, 0, 7]
     coords = (torch.rand(B, N, 3, generator=g, device="cuda") - 0.5) * 6
-    radii, types = torch.ones(B, N, device="cuda"), torch.randint(0, V, (B, N), generator=g, device="cuda").float()
+    radii, types = torch.ones(B, C if by_type else N, device="cuda"), torch.randint(0, V, (B, N), generator=g, device="cuda").float()
     m = Shifted(V, C)
     up, v = normal(g, B, *gm.grid_dimensions(C)), normal(g, B, N, 3)
 
     def forces(b, n, c, counted):
-        out = lmg.Coords2Grid(gm, types=m)(c, types if counted else types[b, :n], radii if counted else radii[b, :n],
+        out = lmg.Coords2Grid(gm, types=m)(c, types if counted else types[b, :n], radii if counted else radii[b] if by_type else radii[b, :n],
                                            *([counted] if counted else []))
         up_ = (up if counted else up[b]).clone().requires_grad_()
         f, = torch.autograd.grad(out, c, up_, create_graph=True)
@@ -315,7 +318,9 @@ def test_padding_and_second_derivatives():
 
     one = [forces(b, n, coords[b, :n].clone().requires_grad_(), None) for b, n in enumerate(na) if n]
     for b, n in enumerate(na):
-        coords[b, n:], radii[b, n:] = float("nan"), float("nan")
+        coords[b, n:] = float("nan")
+        if not by_type:
+            radii[b, n:] = float("nan")
     all_up, all_shift = forces(0, 0, coords.clone().requires_grad_(), na)
     for (u, _), b in zip(one, (0, 2)):
         torch.testing.assert_close(all_up[b], u, rtol=1e-4, atol=1e-3)
